@@ -94,6 +94,23 @@ class IgcPlane(ctypes.Structure):  # app_core.c:1775 plane
                 ("enter_gain", ctypes.c_float), ("leave_gain", ctypes.c_float)]
 
 
+class IgcPack(ctypes.Structure):  # include/igllm_cuda.h igc_pack
+    _fields_ = [("key_codes", ctypes.c_void_p), ("key_scales", ctypes.c_void_p), ("value_codes", ctypes.c_void_p),
+                ("value_scales", ctypes.c_void_p), ("slot_count", ctypes.c_int), ("head_count", ctypes.c_int),
+                ("position_count", ctypes.c_int), ("head_size", ctypes.c_int), ("device", ctypes.c_int),
+                ("trouble", ctypes.c_void_p)]
+
+
+class IgcPackRows(ctypes.Structure):
+    _fields_ = [("count", ctypes.c_int), ("row_count", ctypes.c_int), ("rows_most", ctypes.c_int),
+                ("start_list", ctypes.c_void_p), ("fill_list", ctypes.c_void_p), ("slot_list", ctypes.c_void_p)]
+
+
+class IgcPackData(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("real_type", ctypes.c_int), ("row_stride", ctypes.c_ssize_t),
+                ("head_stride", ctypes.c_ssize_t)]
+
+
 KEEP_PROMPT = 0  # app_core.c:367
 KEEP_TALK = 1    # app_core.c:368
 KEEP_RUNS = 16   # app_core.c:385
@@ -189,6 +206,12 @@ def _lib():
         "igc_session_cache_room": (ctypes.c_size_t, [vp]),
         "igc_session_cache_room_at": (ctypes.c_size_t, [vp, i]),
         "igc_model_memory_bytes": (ctypes.c_size_t, [vp]),
+        "igc_pack_write": (i, [_P(IgcPack), _P(IgcPackRows), _P(IgcPackData), _P(IgcPackData), vp]),
+        "igc_pack_read": (i, [_P(IgcPack), _P(IgcPackRows), _P(IgcPackData), _P(IgcPackData), vp]),
+        "igc_pack_attend_room": (i, [_P(IgcPack), _P(IgcPackRows), i, i, i, i, _P(ctypes.c_size_t)]),
+        "igc_pack_attend": (i, [_P(IgcPack), _P(IgcPackRows), i, _P(IgcPackData), _P(IgcPackData), i, i,
+                                ctypes.c_float, vp, ctypes.c_size_t, vp]),
+        "igc_pack_status": (i, [_P(IgcPack), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -217,6 +240,7 @@ def exported_symbols():
         "igc_session_save", "igc_session_load", "igc_session_ids", "igc_keep_note_share",
         "igc_model_cache_scale", "igc_session_cache_peak", "igc_session_cache_room", "igc_session_cache_room_at",
         "igc_model_memory_bytes",
+        "igc_pack_write", "igc_pack_read", "igc_pack_attend_room", "igc_pack_attend", "igc_pack_status",
     ]
 
 
@@ -592,6 +616,146 @@ def norm_rms_fixed(x, w, eps, device=0):
         raise IgcError(code, f"norm_rms_fixed: {len(x)} floats exceed the fixed array's {FIXED_NORM_LIMIT}")
     _check(code, "norm_rms_fixed")
     return out
+
+
+PACK_GROUP = 32  # columns that share a scale
+PACK_TILE = 64   # a slot's positions are a multiple of this
+
+
+class PackCache:
+    """A key/value cache of 4-bit codes (include/igllm_cuda.h igc_pack) in CUDA
+    tensors of torch: `key_codes` and `value_codes` uint8 [slots, heads,
+    positions, size / 2], `key_scales` and `value_scales` float16 [slots, heads,
+    positions, size / 32], contiguous, on one device.  The calls queue their
+    work on that device's current stream of torch and do not wait for it.
+
+    A call's rows: `fill` (int32, one a sequence) is the position of each
+    sequence's first row; `starts` (int32, one more) its first row and the
+    next's, or None where all have equally many; `slots` (int32) its slot, or
+    None for the sequence's own number; `rows_most` the most rows of any
+    sequence (None: all rows).  These are CUDA tensors that the kernels read.
+    Rows of no sequence are left as they are, rows at negative positions are
+    padding, and what does not fit the cache is left out and told by status()."""
+
+    def __init__(self, key_codes, key_scales, value_codes, value_scales):
+        import torch
+        self._torch = torch
+        self._types = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+        if key_codes.dim() != 4:
+            raise ValueError("PackCache: codes are [slots, heads, positions, size / 2]")
+        slots, heads, positions, half = key_codes.shape
+        for name, t, kind, last in (("key_codes", key_codes, torch.uint8, half),
+                                    ("key_scales", key_scales, torch.float16, 2 * half // PACK_GROUP),
+                                    ("value_codes", value_codes, torch.uint8, half),
+                                    ("value_scales", value_scales, torch.float16, 2 * half // PACK_GROUP)):
+            if t.dtype != kind or tuple(t.shape) != (slots, heads, positions, last) or not t.is_contiguous():
+                raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)}, not a contiguous {kind} "
+                                 f"{(slots, heads, positions, last)}")
+            if t.device != key_codes.device or t.device.type != "cuda":
+                raise ValueError(f"PackCache: {name} is on {t.device}")
+        self.device = key_codes.device
+        self.slots, self.heads, self.positions, self.size = slots, heads, positions, 2 * half
+        self.key_codes, self.key_scales = key_codes, key_scales
+        self.value_codes, self.value_scales = value_codes, value_scales
+        self._trouble = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._p = IgcPack(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
+                          value_scales.data_ptr(), slots, heads, positions, 2 * half, self.device.index,
+                          self._trouble.data_ptr())
+        self._room = {}  # scratch bytes by a call's sizes
+        if positions % PACK_TILE or self.size % PACK_GROUP or not PACK_GROUP <= self.size <= 512:
+            raise ValueError(f"PackCache: {positions} positions (a multiple of {PACK_TILE}) of {self.size} values "
+                             f"(a multiple of {PACK_GROUP} up to 512)")
+
+    @classmethod
+    def open(cls, slots, heads, positions, size, device=0):
+        """A cleared cache with room for `positions` (rounded up to 64) a slot."""
+        import torch
+        positions = -(-int(positions) // PACK_TILE) * PACK_TILE
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+
+        def codes():
+            return torch.full((slots, heads, positions, size // 2), 0x88, dtype=torch.uint8, device=dev)
+
+        def scales():
+            return torch.zeros((slots, heads, positions, size // PACK_GROUP), dtype=torch.float16, device=dev)
+
+        return cls(codes(), scales(), codes(), scales())
+
+    def _list(self, t, name, n):
+        if t is None:
+            return None
+        if t.dtype != self._torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or \
+                t.device != self.device:
+            raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not {n} int32 on "
+                             f"{self.device}")
+        return t.data_ptr()
+
+    def _rows(self, rows, fill, starts, slots, rows_most):
+        n = fill.shape[0]
+        return IgcPackRows(n, rows, 0 if rows_most is None else int(rows_most), self._list(starts, "starts", n + 1),
+                           self._list(fill, "fill", n), self._list(slots, "slots", n))
+
+    def _data(self, t, name, rows, heads):
+        if t.shape != (rows, heads, self.size) or t.device != self.device or t.dtype not in self._types:
+            raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not rows of "
+                             f"{(rows, heads, self.size)} on {self.device}")
+        row, head, last = t.stride()
+        if last != 1 and t.numel():
+            raise ValueError(f"PackCache: the values of a head of {name} are not adjacent")
+        return IgcPackData(t.data_ptr(), self._types[t.dtype], row, head)
+
+    def _stream(self):
+        return self._torch.cuda.current_stream(self.device).cuda_stream
+
+    def write(self, keys, values, fill, starts=None, slots=None, rows_most=None):
+        """Rows [n, heads, size] quantised into their places."""
+        n = keys.shape[0]
+        if n == 0:
+            return
+        _check(_lib().igc_pack_write(self._p, self._rows(n, fill, starts, slots, rows_most),
+                                     self._data(keys, "keys", n, self.heads),
+                                     self._data(values, "values", n, self.heads), self._stream()), "pack_write")
+
+    def read(self, fill, rows, dtype, starts=None, slots=None, rows_most=None, out=None):
+        """(keys, values) of `rows` rows decoded, [rows, heads, size] of `dtype`
+        (in arrays made here, rows of no sequence hold nothing of meaning)."""
+        if out is None:
+            out = tuple(self._torch.empty((rows, self.heads, self.size), dtype=dtype, device=self.device) for _ in range(2))
+        if rows:
+            _check(_lib().igc_pack_read(self._p, self._rows(rows, fill, starts, slots, rows_most),
+                                        self._data(out[0], "keys", rows, self.heads),
+                                        self._data(out[1], "values", rows, self.heads), self._stream()), "pack_read")
+        return out
+
+    def attend(self, queries, fill, starts=None, slots=None, window=0, sinks=0, scale=1.0, rows_most=None, out=None):
+        """Attention of query rows [n, query heads, size] over the cache: row i of
+        a sequence, at fill + i, sees every position up to its own, with a window
+        only the last `window` of them and the first `sinks` of all."""
+        n, heads = queries.shape[0], queries.shape[1]
+        if out is None:
+            out = self._torch.empty(queries.shape, dtype=queries.dtype, device=queries.device)
+        if n == 0:
+            return out
+        rows = self._rows(n, fill, starts, slots, rows_most)
+        q, o = self._data(queries, "queries", n, heads), self._data(out, "out", n, heads)
+        key = (n, rows.count, rows.rows_most, starts is None, heads, q.real_type, window, sinks)
+        room = self._room.get(key)
+        if room is None:
+            need = ctypes.c_size_t()
+            _check(_lib().igc_pack_attend_room(self._p, rows, heads, q.real_type, window, sinks, need),
+                   "pack_attend_room")
+            if len(self._room) > 4096:
+                self._room.clear()
+            room = self._room[key] = need.value
+        work = self._torch.empty(room, dtype=self._torch.uint8, device=self.device) if room else None
+        _check(_lib().igc_pack_attend(self._p, rows, heads, q, o, window, sinks, scale,
+                                      work.data_ptr() if room else None, room, self._stream()), "pack_attend")
+        return out
+
+    def status(self):
+        """Waits for the current stream; raises IgcError (FAIL_STATE) where a call
+        since the last status met rows that do not fit the cache."""
+        _check(_lib().igc_pack_status(self._p, self._stream()), "pack_status")
 
 
 def synth_write(spec, folder, threads=8):

@@ -1,0 +1,72 @@
+// igc_pack.h - host-side launchers of igc_pack.cu: the 4-bit key/value cache.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace igc {
+
+constexpr int PACK_GROUP = 32;  // columns that share a scale
+constexpr int PACK_TILE = 64;   // positions a tile; a slot holds a whole number of them
+
+// A packed cache in device memory: codes [slot][head][position][size / 2]
+// bytes, scales [slot][head][position][size / 32] f16.
+struct PackView {
+  uint8_t *kc, *vc;
+  uint16_t *ks, *vs;
+  int slots, heads, positions, size;
+  int *trouble;  // set nonzero where a call names a place outside the cache (nullable)
+};
+
+// The rows of a call: sequence s has rows [starts[s], starts[s + 1]) (or, with
+// no starts, s * per .. + per), at positions fill[s] + i of slot slots[s] (or s).
+// No sequence has more than `most`.
+struct PackRows {
+  int count, rows, per, most;
+  const int *starts, *fill, *slots;
+};
+
+// Rows of values, `type` 1 f32, 2 f16, 3 bf16; strides in values.
+struct PackData {
+  void *data;
+  int type;
+  long row_stride, head_stride;
+};
+
+struct PackAttend {
+  PackView c;
+  PackRows r;
+  PackData q, out;
+  int group;          // query heads a key/value head
+  int window, sinks;  // window 0: every position up to the row's own
+  float scale;
+  float *work;        // split units' partial sums (PackPlan::work_floats)
+};
+
+// How a call's attention runs, from its host-known sizes alone.
+struct PackPlan {
+  int tiles16;   // 16-row tiles a block holds (1, 2 or 4)
+  int wide;      // head width the kernel is built for: 64, 128, 256 or 512
+  int split2;    // f32 rows: hi and lo halves of both operands
+  int blocks;    // blocks a sequence can need, at most
+  int spread;    // 1: one list of tiles over all units, an equal share a block; 0: `parts` blocks a unit
+  int parts;
+  int grid;
+  int units;     // (block, key/value head) units the grid and the merge cover
+  size_t work_floats;
+};
+
+}  // namespace igc
+
+extern "C" {
+cudaError_t igc_launch_pack_write(const igc::PackView *c, const igc::PackRows *r, const igc::PackData *k,
+                                  const igc::PackData *v, cudaStream_t st);
+cudaError_t igc_launch_pack_read(const igc::PackView *c, const igc::PackRows *r, const igc::PackData *k,
+                                 const igc::PackData *v, cudaStream_t st);
+// `type` the query rows' type, `rows_most` the most rows of any sequence.
+cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int kv_heads, int group, int size,
+                          int type, int window, int sinks, igc::PackPlan *plan);
+cudaError_t igc_launch_pack_attend(const igc::PackAttend *a, const igc::PackPlan *plan, cudaStream_t st,
+                                   int *launches);
+}

@@ -33,6 +33,7 @@
 #include "igc_json.h"
 #include "igc_kernels.h"
 #include "igc_lanes.h"
+#include "igc_pack.h"
 #include "igc_synth.h"
 
 using namespace igc;
@@ -3279,4 +3280,152 @@ extern "C" int igc_norm_rms_fixed(int device, const float *value_list, const flo
   int c = norm_rms_fixed_on(device, value_list, gain_list, value_count, eps_value, value_out);
   if (before >= 0 && before != device) cudaSetDevice(before);  // the caller's device stays current
   return c;
+}
+
+// ---------------------------------------------------------------------------
+// the packed cache's operators: arguments checked here, kernels in igc_pack.cu
+
+namespace {
+
+struct DeviceScope {  // the pack's device for the call, the caller's after it
+  int before = -1, device;
+  explicit DeviceScope(int d) : device(d) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+  }
+  int enter() {
+    if (before != device) CK(cudaSetDevice(device));
+    return IGC_OKAY;
+  }
+  ~DeviceScope() {
+    if (before >= 0 && before != device) cudaSetDevice(before);
+  }
+};
+
+bool pack_sane(const igc_pack *p) {
+  if (!p || !p->key_codes || !p->key_scales || !p->value_codes || !p->value_scales) return false;
+  if ((((size_t)p->key_codes | (size_t)p->key_scales | (size_t)p->value_codes | (size_t)p->value_scales) & 15) != 0)
+    return false;
+  if (p->slot_count < 1 || p->head_count < 1 || p->position_count < PACK_TILE || p->position_count % PACK_TILE != 0)
+    return false;
+  if (p->head_size < PACK_GROUP || p->head_size > 512 || p->head_size % PACK_GROUP != 0) return false;
+  return p->device >= 0 && p->position_count <= (1 << 30) && p->head_count <= (1 << 16);
+}
+
+bool pack_rows_sane(const igc_pack *p, const igc_pack_rows *r) {
+  if (!r || r->count < 1 || r->row_count < 0 || r->rows_most < 0 || !r->fill_list) return false;
+  if (!r->start_list && r->row_count % r->count != 0) return false;
+  if (!r->slot_list && r->count > p->slot_count) return false;
+  return r->row_count <= (1 << 30) && r->count <= (1 << 24);
+}
+
+bool pack_data_sane(const igc_pack_data *d) {
+  if (!d || !d->data || d->real_type < 1 || d->real_type > 3) return false;
+  if ((size_t)d->data % (d->real_type == 1 ? 4 : 2) != 0) return false;
+  return d->row_stride >= 0 && d->head_stride >= 0;
+}
+
+PackView pack_view(const igc_pack *p) {
+  return PackView{(uint8_t *)p->key_codes,      (uint8_t *)p->value_codes, (uint16_t *)p->key_scales,
+                  (uint16_t *)p->value_scales,  p->slot_count,             p->head_count,
+                  p->position_count,            p->head_size,              p->trouble};
+}
+
+PackRows pack_rows_of(const igc_pack_rows *r) {
+  const int per = r->row_count / r->count;
+  int most = r->rows_most > 0 && r->rows_most < r->row_count ? r->rows_most : r->row_count;
+  if (!r->start_list) most = per;
+  return PackRows{r->count, r->row_count, per, most, r->start_list, r->fill_list, r->slot_list};
+}
+
+PackData pack_data_of(const igc_pack_data *d) {
+  return PackData{d->data, d->real_type, (long)d->row_stride, (long)d->head_stride};
+}
+
+int pack_move(bool write, const igc_pack *p, const igc_pack_rows *rows, const igc_pack_data *k,
+              const igc_pack_data *v, void *stream) {
+  if (!pack_sane(p) || !pack_rows_sane(p, rows) || !pack_data_sane(k) || !pack_data_sane(v)) return IGC_FAIL_ARGUMENT;
+  if (rows->row_count == 0) return IGC_OKAY;
+  clear_stale("pack rows");
+  DeviceScope dev(p->device);
+  if (int c = dev.enter()) return c;
+  const PackView view = pack_view(p);
+  const PackRows r = pack_rows_of(rows);
+  const PackData dk = pack_data_of(k), dv = pack_data_of(v);
+  CKL((write ? igc_launch_pack_write : igc_launch_pack_read)(&view, &r, &dk, &dv, (cudaStream_t)stream));
+  return IGC_OKAY;
+}
+
+bool pack_attend_sane(const igc_pack *p, const igc_pack_rows *rows, int heads, int window, int sinks) {
+  if (!pack_sane(p) || !pack_rows_sane(p, rows) || window < 0 || sinks < 0) return false;
+  if (heads < p->head_count || heads % p->head_count != 0) return false;
+  return (long)rows->row_count * (heads / p->head_count) <= (1L << 30);
+}
+
+int pack_plan_of(const igc_pack *p, const PackRows &r, int heads, int type, int window, int sinks, PackPlan *plan) {
+  CK(igc_pack_plan(r.count, r.rows, r.most, p->position_count, p->head_count, heads / p->head_count, p->head_size, type,
+                   window, sinks, plan));
+  return IGC_OKAY;
+}
+
+}  // namespace
+
+extern "C" int igc_pack_write(const igc_pack *p, const igc_pack_rows *rows, const igc_pack_data *k,
+                              const igc_pack_data *v, void *stream) {
+  return pack_move(true, p, rows, k, v, stream);
+}
+
+extern "C" int igc_pack_read(const igc_pack *p, const igc_pack_rows *rows, const igc_pack_data *k,
+                             const igc_pack_data *v, void *stream) {
+  return pack_move(false, p, rows, k, v, stream);
+}
+
+extern "C" int igc_pack_attend_room(const igc_pack *p, const igc_pack_rows *rows, int heads, int type, int window,
+                                    int sinks, size_t *bytes) {
+  if (!bytes || type < 1 || type > 3 || !pack_attend_sane(p, rows, heads, window, sinks)) return IGC_FAIL_ARGUMENT;
+  *bytes = 0;
+  if (rows->row_count == 0) return IGC_OKAY;
+  clear_stale("pack attend room");
+  DeviceScope dev(p->device);
+  if (int c = dev.enter()) return c;
+  PackPlan plan;
+  if (int c = pack_plan_of(p, pack_rows_of(rows), heads, type, window, sinks, &plan)) return c;
+  *bytes = plan.work_floats * sizeof(float);
+  return IGC_OKAY;
+}
+
+extern "C" int igc_pack_attend(const igc_pack *p, const igc_pack_rows *rows, int heads, const igc_pack_data *q,
+                               const igc_pack_data *out, int window, int sinks, float scale, void *work,
+                               size_t work_bytes, void *stream) {
+  if (!pack_attend_sane(p, rows, heads, window, sinks) || !pack_data_sane(q) || !pack_data_sane(out))
+    return IGC_FAIL_ARGUMENT;
+  if (q->real_type != out->real_type || !std::isfinite(scale) || ((size_t)work & 15) != 0) return IGC_FAIL_ARGUMENT;
+  if (rows->row_count == 0) return IGC_OKAY;
+  clear_stale("pack attend");
+  DeviceScope dev(p->device);
+  if (int c = dev.enter()) return c;
+  const PackRows r = pack_rows_of(rows);
+  PackPlan plan;
+  if (int c = pack_plan_of(p, r, heads, q->real_type, window, sinks, &plan)) return c;
+  if (plan.work_floats * sizeof(float) > work_bytes || (plan.work_floats && !work)) return IGC_FAIL_MEMORY;
+  const PackAttend a = {pack_view(p), r,     pack_data_of(q), pack_data_of(out), heads / p->head_count,
+                        window,       sinks, scale,           (float *)work};
+  int launches = 0;
+  const cudaError_t e = igc_launch_pack_attend(&a, &plan, (cudaStream_t)stream, &launches);
+  g_launches += launches;
+  if (e != cudaSuccess) return fail_device(e, "igc_launch_pack_attend");
+  return IGC_OKAY;
+}
+
+extern "C" int igc_pack_status(const igc_pack *p, void *stream) {
+  if (!pack_sane(p)) return IGC_FAIL_ARGUMENT;
+  DeviceScope dev(p->device);
+  if (int c = dev.enter()) return c;
+  CK(cudaStreamSynchronize((cudaStream_t)stream));
+  if (!p->trouble) return IGC_OKAY;
+  int32_t word = 0;
+  CK(cudaMemcpyAsync(&word, p->trouble, sizeof(word), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+  CK(cudaStreamSynchronize((cudaStream_t)stream));
+  if (word == 0) return IGC_OKAY;
+  CK(cudaMemsetAsync(p->trouble, 0, sizeof(word), (cudaStream_t)stream));
+  return IGC_FAIL_STATE;
 }

@@ -1,14 +1,15 @@
 /* igllm_cuda.h - libigllm_cuda: the B200 backend for the speculative verify
  * round of the Gemma-4-E2B text stack (iamhaymc/igllm, "INFERGEM").
  *
- * A plain C ABI: no C++ types, no device pointers cross it.  Every entry that
+ * A plain C ABI: no C++ types cross it, and device pointers only in the packed
+ * cache's operators (igc_pack_*).  Every entry that
  * has a counterpart in the reference engine names it (file:line in the
  * reference's app_core.c / app_main.c) and keeps its argument meaning and its
  * error behaviour: results are the reference's app_code values, zero for
  * success and negative for failure, and a refused call leaves the session as
  * it was.
  *
- * Two layers are exported.
+ * Three layers are exported.
  *
  *  1. The backend table (`igc_desk`), the device twin of the reference's
  *     `back_desk` (app_core.c:5222-5245): the six entries the engine reaches
@@ -19,6 +20,9 @@
  *     block, its keep and its tempered verify.  The whole pass runs on the
  *     GPU with the weights resident in HBM; only ids go in and only ids (or,
  *     on request, logit rows) come out.
+ *  3. The packed cache's operators (`igc_pack_*`, no counterpart in the
+ *     reference): a key/value cache of 4-bit codes in the caller's device
+ *     memory, written, read back and attended over, on the caller's stream.
  *
  * Threading: one caller at a time per session (the reference's rule,
  * app_core.c:7789-7793).  Separate sessions, and separate models on separate
@@ -334,6 +338,87 @@ int igc_session_stamps(igc_session *session, int k, int *cls_out, double *bytes_
 #define IGC_FIXED_DEVICE_LIMIT 64
 int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_list, int value_count,
                        float eps_value, float *value_out);
+
+/* ---- 3. the packed cache (no counterpart in the reference) ---------------
+ *
+ * A key/value cache in the caller's device memory that holds 4-bit codes:
+ * for each (slot, key/value head, position) `head_size` codes, two a byte, low
+ * nibble first, and one f16 scale for each 32 of them,
+ *
+ *   scale = f16(min(max|x| / 7, 8188)), the quotient in f32,
+ *   code  = clamp(rint(x / scale), -8, 7) + 8,  read back as (code - 8) * scale,
+ *
+ * 0.5625 bytes a value.  Values past 8 * 8188 and infinities saturate; a NaN
+ * is stored as 0.  Codes are [slot][head][position][head_size / 2] bytes,
+ * scales [slot][head][position][head_size / 32] halves, keys and values apart,
+ * each array on a 16-byte boundary; `position_count` is a multiple of 64 and
+ * `head_size` of 32, at most 512.  `trouble`, when not NULL, is a device word
+ * (zero at first) that calls set where what they find on the device does not
+ * fit the cache; igc_pack_status reads and clears it.
+ *
+ * igc_pack_rows names a call's rows: sequence s has rows start_list[s] ..
+ * start_list[s + 1] of the call's arrays (without a start_list, row_count /
+ * count each), and its row i stands at position fill_list[s] + i of slot
+ * slot_list[s] (without one, s).  The lists are device arrays, read when the
+ * kernels run, so a captured call follows them.  rows_most bounds the rows of
+ * any sequence (0: row_count).  Rows no sequence holds are left as they are.
+ * A row at a negative position is padding: not written, and zeros out.  A row
+ * at position_count or beyond, or of a slot the cache lacks, is not written,
+ * comes out as zeros and sets the trouble word; a sequence whose rows fall
+ * outside [0, row_count) or pass rows_most is not run and sets it too.  The
+ * places written by one call are the caller's to keep distinct.
+ *
+ * igc_pack_data is an array of rows: `real_type` 1 F32, 2 F16, 3 BF16 (the
+ * reference's store_type values), strides in values, a head's values adjacent.
+ *
+ * igc_pack_write: keys and values (row_count x head_count x head_size) into
+ * their places.  igc_pack_read: the same places decoded.
+ *
+ * igc_pack_attend: for each row at position p and each of `head_count` query
+ * heads (head h reads key/value head h / (head_count / pack->head_count)),
+ * softmax(scale q.k) over the positions j <= p, with window > 0 only those
+ * with j > p - window or j < sink_count, times the values.  The row's own key
+ * is read from the cache: write it first.  `out` has the queries' type.  Sums
+ * and the softmax are f32; queries are read as f16 after an exact power of two
+ * a row, and for F32 rows every product keeps both halves of a hi/lo split, so
+ * that results hold to f32.  `work` is device scratch of at least the bytes
+ * igc_pack_attend_room gives for the same arguments (a multiple of 16 bytes
+ * aligned); calls that may run at once need scratch of their own.
+ *
+ * Each call makes pack->device current and restores the caller's device; work
+ * is queued on `stream` (a cudaStream_t, NULL the default stream) and not
+ * waited for.  The first call of a form on a device loads it: make it before
+ * a stream capture.  A refused call queues nothing. */
+typedef struct igc_pack {
+  void *key_codes, *key_scales, *value_codes, *value_scales;
+  int slot_count, head_count, position_count, head_size;
+  int device;
+  int32_t *trouble;
+} igc_pack;
+
+typedef struct igc_pack_rows {
+  int count, row_count, rows_most;
+  const int32_t *start_list, *fill_list, *slot_list;
+} igc_pack_rows;
+
+typedef struct igc_pack_data {
+  void *data;
+  int real_type;
+  ptrdiff_t row_stride, head_stride;
+} igc_pack_data;
+
+int igc_pack_write(const igc_pack *pack, const igc_pack_rows *rows, const igc_pack_data *keys,
+                   const igc_pack_data *values, void *stream);
+int igc_pack_read(const igc_pack *pack, const igc_pack_rows *rows, const igc_pack_data *keys_out,
+                  const igc_pack_data *values_out, void *stream);
+int igc_pack_attend_room(const igc_pack *pack, const igc_pack_rows *rows, int head_count, int real_type, int window,
+                         int sink_count, size_t *bytes_out);
+int igc_pack_attend(const igc_pack *pack, const igc_pack_rows *rows, int head_count, const igc_pack_data *queries,
+                    const igc_pack_data *out, int window, int sink_count, float scale, void *work, size_t work_bytes,
+                    void *stream);
+/* Waits for `stream`, then IGC_OKAY, or IGC_FAIL_STATE where a call since the
+ * last status set the trouble word (which is cleared). */
+int igc_pack_status(const igc_pack *pack, void *stream);
 
 /* ---- n-gram scout (app_core.c:12277-12361), host C --------------------- */
 
