@@ -19,8 +19,10 @@
 //   j in [0, p], with a window only j > p - window or j < sinks.
 //
 // Rows at negative positions are padding: not written, and zeros out.
-#include <cuda_fp16.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <string.h>
@@ -143,6 +145,38 @@ __device__ __forceinline__ void store8(void *base, int type, size_t at, bool wid
   }
 }
 
+// Four values; `wide`: eight from any multiple of eight columns start on 16 bytes.
+__device__ __forceinline__ void store4(void *base, int type, size_t at, bool wide, const float (&x)[4]) {
+  if (type == 1) {
+    float *p = static_cast<float *>(base) + at;
+    if (wide) {
+      *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = x[i];
+    }
+    return;
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (type == 2) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+  }
+  uint16_t *p = static_cast<uint16_t *>(base) + at;
+  if (wide) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) p[2 * i] = (uint16_t)w[i], p[2 * i + 1] = (uint16_t)(w[i] >> 16);
+  }
+}
+
 // Whether every group of eight values of these rows starts on 16 bytes.
 __device__ __forceinline__ bool wide_rows(const PackData &d) {
   const long per = d.type == 1 ? 4 : 8;
@@ -236,78 +270,94 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(PackIo a) {
 // ---------------------------------------------------------------------------
 // attention over the codes on mma.sync tiles
 //
-// A block holds RB = 16 MT query rows of one (sequence, key/value head): row
+// A block holds RB = 8 NT query rows of one (sequence, key/value head): row
 // rr is the sequence's row rr / group, head rr % group of the group, so a
-// token's heads share each tile of codes.  Four warps walk tiles of 64
-// positions that cp.async brings three tiles deep:
+// token's heads share each tile of codes.  Four warps walk tiles of 64 MP
+// positions that TMA brings NS deep, swizzled so that the reads below spread
+// over the banks.  Positions and columns are the products' 16 rows and query
+// rows their 8 columns, so eight heads fill a product.
 //
-//   scores  warp w takes positions 16 w .. 16 w + 15.  A code nibble n in the
-//           low bits of a half is the f16 number n 2^-24 (or 16 n 2^-24 four
-//           bits up, its query column kept as q / 16), exact without any
-//           conversion, so a code word costs five integer instructions.  The
-//           -8 of every code is the products' starting accumulator,
-//           -8 sum q over the group; the group's sum times its scale is an
-//           f32 multiply-add.  Which column of a group a thread's product
-//           slot holds is free as long as the query fragments agree.
+//   scores  warp w takes positions 16 MP w on.  A code word becomes eight
+//           n - 8, exact in f16, by nine instructions; which column of a
+//           group a thread's product slot holds is free as long as the query
+//           fragments agree, so words are used as they lie.  A group's sum
+//           times its scale is an f32 multiply-add.  (Nibbles left in place
+//           as subnormal halves, their -8 taken out of the sums, saved four
+//           instructions a word and cost 2^-13 of a scale: the tensor core
+//           aligns products by their exponent fields.)
 //   softmax the running maximum and sum per row in 32 bits; the block's
 //           maximum is merged through shared memory once a tile.
 //   values  warp w takes 64 of the head's columns (or, of a narrow head, a
-//           share of the positions).  A value enters as f16((code - 8) scale),
-//           rounded once (2^-11 at most); pairs of positions are zipped by byte
-//           permutes, so codes are used as they lie, with no transpose.  A
-//           thread ends with 16 consecutive columns of its rows.
+//           share of the positions).  Codes of two positions are zipped by a
+//           byte permute, used as they lie.  For 16-bit rows the group's
+//           scale goes into the weight, f16(f16(w) 8 scale), two roundings of
+//           2^-11 at most, and codes enter exactly.
 //
 // A query row is scaled by the power of two that puts its largest magnitude
 // in [2^13, 2^14) and kept as f16, exact for bf16 and f16 rows but for
-// magnitudes 2^38 below the largest.  Weights are scaled by 2^12 (the sum
-// alike) and rounded to f16, 2^-11 at most each; the results are rounded to 16
-// bits anyway.
-// For f32 rows (SP) queries, weights and values are each kept as f16 hi and lo
-// parts, the products left out (lo x lo) below f32's own rounding.
+// magnitudes 2^38 below the largest.  For f32 rows (SP) queries and weights
+// are each kept as f16 hi and lo parts and (n - 8) scale as hi and lo, which
+// hold it exactly; the products left out (lo x lo) are below f32's own
+// rounding, and each step of 16 positions starts from zero accumulators, as
+// the tensor core's sums round towards zero.
 
-template <int HDP, int MT, bool SP>
+constexpr int PACK_TRIES = 1 << 22;  // polls a wait makes before it gives up
+
+template <int HDP, int NT, bool SP>
 struct PackTile {
-  static constexpr int RB = 16 * MT;
+  static constexpr int RB = 8 * NT;
   static constexpr int C = HDP / 32;                     // groups
-  static constexpr int CB = HDP / 2;                     // code bytes a position
-  static constexpr int NS = 3;                           // tiles in flight
+  static constexpr int PITCH = HDP >= 256 ? 128 : HDP / 2;  // code bytes of a swizzled row
+  static constexpr int HALVES = HDP / 2 / PITCH;         // rows of 512 columns lie in two halves
+  static constexpr int MP = NT <= 2 && HDP <= 256 ? 2 : 1;
+  static constexpr int TP = 64 * MP;                     // positions a step
+  static constexpr int NS = HDP <= 128 ? 3 : MP == 2 || HDP == 512 ? 2 : 3;  // steps in flight
   static constexpr int WC = HDP >= 256 ? 4 : HDP / 64;   // warps across the columns
-  static constexpr int WP = 4 / WC;                      // warps across a tile's positions
+  static constexpr int WP = 4 / WC;                      // warps across a step's positions
   static constexpr int NB = HDP / 64 / WC;               // 64-column blocks a warp
-  static constexpr int SCP = 72;                         // scales a group row (64 and a bank shift)
   static constexpr int PARTS = SP ? 2 : 1;
-  static constexpr int QF = C * 2 * MT * 512;            // bytes of one part's query fragments
-  static constexpr int OFF_QOFF = QF * PARTS;
-  static constexpr int OFF_FR = OFF_QOFF + C * RB * 4;
+  static constexpr int QF = C * NT * 512;                // bytes of one part's query fragments
+  static constexpr int CODE64 = 64 * PITCH;              // one TMA box: 64 positions
+  static constexpr int CODE_SIDE = MP * HALVES * CODE64;
+  static constexpr int SC_SIDE = TP * C * 2;
+  static constexpr int STAGE = 2 * CODE_SIDE + 2 * SC_SIDE;
+  static constexpr int OFF_SC = 2 * CODE_SIDE;           // in a stage: keys, values, key scales, value scales
+  static constexpr int RING = NS * ((STAGE + 1023) / 1024 * 1024);
+  static constexpr int SLOT = RING / NS;
+  static constexpr int OUT_BYTES = WP > 1 ? RB * HDP * 4 : 0;
+  static constexpr int OFF_Q = RING > OUT_BYTES ? RING : OUT_BYTES;
+  static constexpr int OFF_FR = OFF_Q + QF * PARTS;
   static constexpr int OFF_MAX = OFF_FR + RB * 4;
   static constexpr int OFF_SUM = OFF_MAX + 4 * RB * 4;
-  static constexpr int PF = 4 * MT * 512;                // bytes of one part's weight fragments
+  static constexpr int PF = TP / 16 * NT * 256;          // bytes of one part's weight fragments
   static constexpr int OFF_P = OFF_SUM + 4 * RB * 4;
-  static constexpr int OFF_SC = OFF_P + PF * PARTS;      // [NS][key, value][C][SCP] f16
-  static constexpr int SC_SIDE = C * SCP * 2;
-  static constexpr int OFF_CODE = (OFF_SC + NS * 2 * SC_SIDE + 127) / 128 * 128;
-  static constexpr int CODE_SIDE = 64 * CB;
-  static constexpr int OUT_BYTES = WP > 1 ? RB * HDP * 4 : 0;
-  static constexpr int RING = NS * 2 * CODE_SIDE;
-  static constexpr int SMEM = OFF_CODE + (RING > OUT_BYTES ? RING : OUT_BYTES);
+  static constexpr int SMEM = 1024 + OFF_P + PF * PARTS;
+  // blocks an SM that registers are kept for
+  static constexpr int PER_SM = NT == 1 ? (HDP <= 128 ? 4 : 3) : NT == 2 && HDP <= 256 ? 3 : 2;
 };
 
-// 16-byte piece j of position row r sits at piece pk_swz<C>(r, j): rows that
-// share banks keep the same group apart.
-template <int C>
+// Where the 16-byte piece j of position row r lies in a box of PITCH-byte
+// rows: the 128-, 64- and 32-byte swizzles of a tensor map.
+template <int PITCH>
 __device__ __forceinline__ int pk_swz(int r, int j) {
-  if (C >= 8) return j ^ (r & 7);
-  if (C == 4) return j ^ ((r >> 1) & 3);
-  return j ^ ((r >> 2) & 1);
+  if (PITCH == 128) return r * 128 + ((j ^ (r & 7)) << 4);
+  if (PITCH == 64) return r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
+  return r * 32 + ((j ^ ((r >> 2) & 1)) << 4);
 }
 
-__device__ __forceinline__ void cp16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// One box of a code array: 64 rows from row y, PITCH bytes from byte x.
+__device__ __forceinline__ void pk_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -318,6 +368,18 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t y) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// c s - p, exact where p is c s rounded
+__device__ __forceinline__ uint32_t rest2(uint32_t c, uint32_t s, uint32_t p) {
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2 *>(&c), *reinterpret_cast<const __half2 *>(&s),
+                            __hneg2(*reinterpret_cast<const __half2 *>(&p)));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
 // The tiles a block of rows [t0, t1] (of a sequence) reads: tiles [0, head)
 // of the first positions, then [from, from + rest).
@@ -328,22 +390,22 @@ struct TileSpan {
   __device__ __forceinline__ int tile(int k) const { return k < head ? k : from + (k - head); }
 };
 
-__device__ __forceinline__ TileSpan span_of(const PackAttend &a, const SeqAt &q, int t0, int t1) {
+__device__ __forceinline__ TileSpan span_of(const PackAttend &a, const SeqAt &q, int t0, int t1, int tp) {
   TileSpan s = {0, 0, 0, 0, 0};
   const int p0 = max(q.fill + t0, 0), p1 = min(q.fill + t1, a.c.positions - 1);
   if (q.slot < 0 || p1 < p0) return s;
   s.hi = p1 + 1;
   s.lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
-  s.from = s.lo / PACK_TILE;
-  s.rest = (s.hi + PACK_TILE - 1) / PACK_TILE - s.from;
-  s.head = min((min(a.sinks, s.hi) + PACK_TILE - 1) / PACK_TILE, s.from);
+  s.from = s.lo / tp;
+  s.rest = (s.hi + tp - 1) / tp - s.from;
+  s.head = min((min(a.sinks, s.hi) + tp - 1) / tp, s.from);
   return s;
 }
 
 // Block b (of RB rows) of a sequence: its tokens.
-__device__ __forceinline__ TileSpan block_span(const PackAttend &a, const SeqAt &q, int b, int rb) {
+__device__ __forceinline__ TileSpan block_span(const PackAttend &a, const SeqAt &q, int b, int rb, int tp) {
   const int t0 = b * rb / a.group, t1 = min(q.n - 1, ((b + 1) * rb - 1) / a.group);
-  return span_of(a, q, t0, t1);
+  return span_of(a, q, t0, t1, tp);
 }
 
 __device__ __forceinline__ int blocks_of(const PackAttend &a, const SeqAt &q, int rb) {
@@ -385,13 +447,13 @@ __device__ __forceinline__ int block_scan(int v, int *red, int *total) {
 
 // A sequence's weight in the list that blocks share out: its tiles over all
 // its blocks and key/value heads (spread), or its blocks.
-__device__ __forceinline__ int seq_weight(const PackAttend &a, int s, int rb, bool spread) {
+__device__ __forceinline__ int seq_weight(const PackAttend &a, int s, int rb, int tp, bool spread) {
   if (s >= a.r.count) return 0;
   const SeqAt q = seq_at(a.c, a.r, s);
   const int nb = blocks_of(a, q, rb);
   if (!spread) return nb;
   int w = 0;
-  for (int b = 0; b < nb; ++b) w += block_span(a, q, b, rb).count();
+  for (int b = 0; b < nb; ++b) w += block_span(a, q, b, rb, tp).count();
   return w * a.c.heads;
 }
 
@@ -400,13 +462,13 @@ __device__ __forceinline__ int seq_weight(const PackAttend &a, int s, int rb, bo
 struct ListAt {
   int total, s, before;
 };
-__device__ __forceinline__ ListAt list_at(const PackAttend &a, int rb, bool spread, int want, int *red) {
+__device__ __forceinline__ ListAt list_at(const PackAttend &a, int rb, int tp, bool spread, int want, int *red) {
   ListAt at = {0, -1, 0};
   int *found = red + 8;
   if (threadIdx.x == 0) found[0] = -1;
   for (int base = 0; base < a.r.count; base += blockDim.x) {
     int t;
-    const int w = seq_weight(a, base + threadIdx.x, rb, spread);
+    const int w = seq_weight(a, base + threadIdx.x, rb, tp, spread);
     const int before = at.total + block_scan(w, red, &t);
     if (want >= before && want - before < w) {
       found[0] = base + threadIdx.x;
@@ -421,10 +483,10 @@ __device__ __forceinline__ ListAt list_at(const PackAttend &a, int rb, bool spre
   return at;
 }
 // The weight of all sequences, and of those before `s`.
-__device__ __forceinline__ int list_total(const PackAttend &a, int rb, bool spread, int s, int *before, int *red) {
+__device__ __forceinline__ int list_total(const PackAttend &a, int rb, int tp, bool spread, int s, int *before, int *red) {
   int w = 0, b = 0;
   for (int i = threadIdx.x; i < a.r.count; i += blockDim.x) {
-    const int x = seq_weight(a, i, rb, spread);
+    const int x = seq_weight(a, i, rb, tp, spread);
     w += x;
     if (i < s) b += x;
   }
@@ -438,42 +500,75 @@ __device__ __forceinline__ int share_of(int total, int grid) {
   return max(PACK_SHARE_LEAST, (total + grid - 1) / grid);
 }
 
-template <int HDP, int MT, bool SP>
-__global__ void __launch_bounds__(128) pack_attend_kernel(PackAttend a, int spread, int parts) {
-  using L = PackTile<HDP, MT, SP>;
-  constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, SCP = L::SCP;
-  extern __shared__ __align__(128) uint8_t sm[];
+
+// What each of `grid` blocks takes of the list (its total in at->total), and
+// where in it block `mine` begins: one pass over the sequences where they fit
+// the block, else two.
+__device__ __forceinline__ int list_share(const PackAttend &a, int rb, int tp, int grid, int mine, ListAt *at,
+                                          int *red) {
+  if (a.r.count <= (int)blockDim.x) {
+    int *found = red + 8;
+    if (threadIdx.x == 0) found[0] = -1;
+    const int w = seq_weight(a, threadIdx.x, rb, tp, true);
+    const int before = block_scan(w, red, &at->total);
+    const int share = share_of(at->total, grid), want = mine * share;
+    if (want >= before && want - before < w) {
+      found[0] = threadIdx.x;
+      found[1] = before;
+    }
+    __syncthreads();
+    at->s = found[0];
+    at->before = found[1];
+    return share;
+  }
+  const int total = list_total(a, rb, tp, true, 0, nullptr, red), share = share_of(total, grid);
+  *at = list_at(a, rb, tp, true, mine * share, red);
+  at->total = total;
+  return share;
+}
+
+template <int HDP, int NT, bool SP>
+__global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
+    pack_attend_kernel(const __grid_constant__ PackAttend a, const __grid_constant__ CUtensorMap tmk,
+                       const __grid_constant__ CUtensorMap tmv, int spread, int parts) {
+  using L = PackTile<HDP, NT, SP>;
+  constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, MP = L::MP, TP = L::TP,
+                PITCH = L::PITCH;
+  extern __shared__ __align__(1024) uint8_t sm_raw[];
   __shared__ int red[16];
-  float *qoff = reinterpret_cast<float *>(sm + L::OFF_QOFF);
+  __shared__ uint64_t full[NS];
+  uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
   float *fr = reinterpret_cast<float *>(sm + L::OFF_FR);
   float *wmax = reinterpret_cast<float *>(sm + L::OFF_MAX);
   float *wsum = reinterpret_cast<float *>(sm + L::OFF_SUM);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const int size = a.c.size, chd = size / 32, group = a.group;
   const int wc = warp % WC, wp = warp / WC;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
+    mbar_init_fence();
+  }
 
-  pdl_wait();
   // which tiles this block takes
-  int at = 0, end = 0, s = 0, b = 0, h = 0, part = 0, share = 0;
+  int at = 0, end = 0, s = 0, b = 0, h = 0, part = 0;
   SeqAt q;
   if (spread) {
-    const int total = list_total(a, RB, true, 0, nullptr, red);
-    share = share_of(total, gridDim.x);
+    ListAt f;
+    const int share = list_share(a, RB, TP, gridDim.x, blockIdx.x, &f, red);
     at = blockIdx.x * share;
-    end = min(total, at + share);
+    end = min(f.total, at + share);
     pdl_release();
     if (at >= end) return;
-    const ListAt f = list_at(a, RB, true, at, red);
     s = f.s;
     if (s < 0) return;
     q = seq_at(a.c, a.r, s);
     int left = at - f.before;
     for (;; ++b) {
       if (b >= blocks_of(a, q, RB)) return;
-      const int n = block_span(a, q, b, RB).count() * a.c.heads;
+      const int n = block_span(a, q, b, RB, TP).count() * a.c.heads;
       if (left < n) {
         h = left / (n / a.c.heads);
-        part = left - h * (n / a.c.heads);  // the tile of the unit it starts at
+        part = left - h * (n / a.c.heads);  // the step of the unit it starts at
         break;
       }
       left -= n;
@@ -482,19 +577,21 @@ __global__ void __launch_bounds__(128) pack_attend_kernel(PackAttend a, int spre
     const int u = blockIdx.x / parts;
     part = blockIdx.x - u * parts;
     h = u % a.c.heads;
-    const int total = list_total(a, RB, false, 0, nullptr, red);
+    const int total = list_total(a, RB, TP, false, 0, nullptr, red);
     const int vb = total - 1 - u / a.c.heads;  // the rows at the end see the most: first
     pdl_release();
     if (vb < 0) return;
-    const ListAt f = list_at(a, RB, false, vb, red);
+    const ListAt f = list_at(a, RB, TP, false, vb, red);
     s = f.s;
     if (s < 0) return;
     b = vb - f.before;
     q = seq_at(a.c, a.r, s);
   }
 
+  int step0 = 0;  // steps this block has taken: the ring's place
+  bool gave_up = false;
   for (;;) {  // one unit, or a piece of it, a turn
-    const TileSpan sp = block_span(a, q, b, RB);
+    const TileSpan sp = block_span(a, q, b, RB, TP);
     const int n = sp.count();
     int ka, kb;
     bool whole;
@@ -511,9 +608,31 @@ __global__ void __launch_bounds__(128) pack_attend_kernel(PackAttend a, int spre
       place = blockIdx.x;
       if (!whole && ka == kb) return;
     }
+    const size_t unit = ((size_t)max(q.slot, 0) * a.c.heads + h) * a.c.positions;
+    // step k's codes and scales: 64 positions a copy, those past the last
+    // position any row sees left out
+    auto load = [&](int k) {
+      if (k >= kb || tid != 0) return;
+      const int i = (step0 + k - ka) % NS, p0 = sp.tile(k) * TP;
+      const int boxes = min(MP, (sp.hi - p0 + 63) / 64);
+      uint8_t *st = sm + i * L::SLOT;
+      const uint32_t scales = (uint32_t)boxes * 64 * chd * 2;
+      mbar_expect(&full[i], (uint32_t)boxes * 2 * L::HALVES * L::CODE64 + 2 * scales);
+      for (int x = 0; x < boxes; ++x)
+#pragma unroll
+        for (int y = 0; y < L::HALVES; ++y) {
+          pk_load(st + (x * L::HALVES + y) * L::CODE64, &tmk, y * 128, (int)unit + p0 + 64 * x, &full[i]);
+          pk_load(st + L::CODE_SIDE + (x * L::HALVES + y) * L::CODE64, &tmv, y * 128, (int)unit + p0 + 64 * x,
+                  &full[i]);
+        }
+      const uint64_t once = l2_evict_first();
+      bulk_load(st + L::OFF_SC, a.c.ks + (unit + p0) * chd, scales, &full[i], once);
+      bulk_load(st + L::OFF_SC + L::SC_SIDE, a.c.vs + (unit + p0) * chd, scales, &full[i], once);
+    };
+    __syncthreads();  // the unit before is done with the ring and the fragments
+    for (int k = ka; k < ka + NS - 1; ++k) load(k);
 
     // ---- the query rows, as fragments
-    __syncthreads();
     {
       const bool wide = wide_rows(a.q);
       constexpr int WPL = HDP >= 256 ? HDP / 256 : 1;  // code words a lane
@@ -541,502 +660,526 @@ __global__ void __launch_bounds__(128) pack_attend_kernel(PackAttend a, int spre
           frexpf(big, &ex);
           ex = 14 - ex;  // big 2^ex in [2^13, 2^14)
         }
-        if (lane == 0) fr[r] = ldexpf(a.scale * 1.4426950408889634f, 24 - ex);
+        const float up0 = pow2i(ex / 2), up1 = pow2i(ex - ex / 2);
+        if (lane == 0) fr[r] = ldexpf(a.scale * 1.4426950408889634f, -ex);
 #pragma unroll
         for (int i = 0; i < WPL; ++i) {
           const int w = lane + 32 * i, gq = w >> 2, tq = w & 3;
           if (w >= HDP / 8) continue;  // narrow heads: the lanes past the row
-          float sum = 0.0f, y[8], z[8];
+          float y[8], z[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float v = ldexpf(x[i][e], ex);
-            const float hi = __half2float(__float2half_rn(v));
-            y[e] = hi;
-            z[e] = SP ? __half2float(__float2half_rn(v - hi)) : 0.0f;
-            sum += SP ? y[e] + z[e] : y[e];
+            const float v = x[i][e] * up0 * up1;
+            y[e] = __half2float(__float2half_rn(v));
+            z[e] = v - y[e];
           }
-          const uint32_t four = 0xfu << (lane & 28);
-          sum += __shfl_xor_sync(four, sum, 1);
-          sum += __shfl_xor_sync(four, sum, 2);
-          if (tq == 0) qoff[gq * RB + r] = -8.0f * 5.9604644775390625e-08f * sum;  // 2^-24
-          // product m of a group: columns (2m, 2m + 4) and, an 1/16th of them, (2m + 1, 2m + 5)
+          // product m of a group: columns (2m, 2m + 4) and (2m + 1, 2m + 5)
 #pragma unroll
           for (int pt = 0; pt < L::PARTS; ++pt) {
             const float(&v)[8] = pt ? z : y;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              uint32_t *f = reinterpret_cast<uint32_t *>(sm + pt * L::QF) +
-                            (((gq * 2 + m) * MT + (r >> 4)) * 32 + (r & 7) * 4 + tq) * 4 + ((r & 8) ? 1 : 0);
-              f[0] = half2_bits(v[2 * m], v[2 * m + 4]);
-              f[2] = half2_bits(v[2 * m + 1] * 0.0625f, v[2 * m + 5] * 0.0625f);
-            }
+            reinterpret_cast<uint4 *>(sm + L::OFF_Q + pt * L::QF)[(gq * NT + (r >> 3)) * 32 + (r & 7) * 4 + tq] =
+                make_uint4(half2_bits(v[0], v[4]), half2_bits(v[1], v[5]), half2_bits(v[2], v[6]),
+                           half2_bits(v[3], v[7]));
           }
         }
       }
-      // groups past the head: their scales stay zero
-      for (int i = tid; i < NS * 2 * (C - chd) * SCP; i += 128) {
-        const int st = i / ((C - chd) * SCP), e = i - st * (C - chd) * SCP;
-        reinterpret_cast<uint16_t *>(sm + L::OFF_SC + st * L::SC_SIDE)[chd * SCP + e] = 0;
-      }
     }
-    int pos[MT][2];  // the position of this thread's rows, -1 for none
+    int pos[NT][2];  // the position of this thread's rows, -1 for none
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int rr = b * RB + mt * 16 + g8 + 8 * e, p = q.fill + rr / group;
-        pos[mt][e] = rr < q.n * group && p < a.c.positions ? max(p, -1) : -1;
+        const int rr = b * RB + nt * 8 + 2 * t4 + e, p = q.fill + rr / group;
+        pos[nt][e] = rr < q.n * group && p < a.c.positions ? max(p, -1) : -1;
       }
     const int p_first = q.fill + b * RB / group;  // the first row's
     const int p_last = sp.hi - 1;
     const bool past = q.fill + min(q.n - 1, ((b + 1) * RB - 1) / group) >= a.c.positions;
-
     if (tid == 0 && (past || q.slot < 0)) pack_trouble(a.c);
+    __syncthreads();
 
     // ---- the tiles
-    const size_t unit = ((size_t)max(q.slot, 0) * a.c.heads + h) * a.c.positions;
-    const uint8_t *kc = a.c.kc + unit * (size / 2), *vc = a.c.vc + unit * (size / 2);
-    const uint16_t *scp = (tid >= 64 ? a.c.vs : a.c.ks) + unit * chd;
-    uint32_t screg[C / 2];
-    auto load_codes = [&](int k) {
-      if (k < kb) {
-        const size_t from = (size_t)sp.tile(k) * PACK_TILE * (size / 2);
-        uint8_t *dk = sm + L::OFF_CODE + (k % NS) * 2 * L::CODE_SIDE, *dv = dk + L::CODE_SIDE;
-        if (chd == C) {
+    float o[NT][NB * 4][4];  // [16 columns: two of them a thread][column, query row]
+    float m_run[NT][2], l_run[NT][2];
 #pragma unroll
-          for (int i = 0; i < 64 * C / 128; ++i) {
-            const int e = tid + 128 * i, r = e / C, j = e % C, o = r * L::CB + pk_swz<C>(r, j) * 16;
-            cp16(dk + o, kc + from + (size_t)e * 16);
-            cp16(dv + o, vc + from + (size_t)e * 16);
-          }
-        } else {
-          for (int e = tid; e < 64 * chd; e += 128) {
-            const int r = e / chd, j = e - r * chd, o = r * L::CB + pk_swz<C>(r, j) * 16;
-            cp16(dk + o, kc + from + (size_t)e * 16);
-            cp16(dv + o, vc + from + (size_t)e * 16);
-          }
-        }
-      }
-      cp_commit();
-    };
-    // scales pass through registers: position tid % 64's of the key side
-    // (first half of the block) or the value side
-    auto load_scales = [&](int k) {
-      if (k >= kb) return;
-      const uint16_t *src = scp + ((size_t)sp.tile(k) * PACK_TILE + (tid & 63)) * chd;
-      if (chd == C) {
-        if constexpr (C == 2) screg[0] = *reinterpret_cast<const uint32_t *>(src);
-        else if constexpr (C == 4) *reinterpret_cast<uint2 *>(screg) = *reinterpret_cast<const uint2 *>(src);
-        else {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int i = 0; i < C / 8; ++i)
-            reinterpret_cast<uint4 *>(screg)[i] = reinterpret_cast<const uint4 *>(src)[i];
-        }
-      } else {
+      for (int e = 0; e < 2; ++e) m_run[nt][e] = -INFINITY, l_run[nt][e] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < C / 2; ++i)
-          screg[i] = (2 * i < chd ? (uint32_t)src[2 * i] : 0u) | (2 * i + 1 < chd ? (uint32_t)src[2 * i + 1] << 16 : 0u);
-      }
-    };
-    auto keep_scales = [&](int k) {
-      if (k >= kb) return;
-      const int r = tid & 63, p = sp.tile(k) * PACK_TILE + r;
-      // a value no row of the block sees counts as 0 whatever lies there
-      const bool seen = p < sp.hi && (p >= sp.lo || p < a.sinks);
-      uint16_t *dst = reinterpret_cast<uint16_t *>(sm + L::OFF_SC + ((k % NS) * 2 + (tid >> 6)) * L::SC_SIDE) + r;
+      for (int j = 0; j < NB * 4; ++j)
 #pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (i < chd) dst[i * SCP] = seen ? (uint16_t)(screg[i >> 1] >> (16 * (i & 1))) : (uint16_t)0;
-    };
-
-    float o[MT][NB * 8][4];
-    float m_run[MT][2], l_run[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) m_run[mt][e] = -INFINITY, l_run[mt][e] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NB * 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.0f;
     }
-    load_codes(ka);
-    load_scales(ka);
-    keep_scales(ka);
-    load_codes(ka + 1);
-    load_scales(ka + 1);
     for (int k = ka; k < kb; ++k) {
-      cp_wait<1>();
-      __syncthreads();
-      keep_scales(k + 1);
-      load_codes(k + 2);
-      load_scales(k + 2);
-      const uint8_t *tk = sm + L::OFF_CODE + (k % NS) * 2 * L::CODE_SIDE, *tv = tk + L::CODE_SIDE;
-      const uint16_t *ksc = reinterpret_cast<const uint16_t *>(sm + L::OFF_SC + (k % NS) * 2 * L::SC_SIDE);
-      const uint16_t *vsc = ksc + L::SC_SIDE / 2;
+      const int turn = step0 + k - ka, slot = turn % NS;
+      gave_up = !mbar_wait(&full[slot], (uint32_t)((turn / NS) & 1), gave_up ? PACK_TRIES / 64 : PACK_TRIES) || gave_up;
+      const uint8_t *tk = sm + slot * L::SLOT, *tv = tk + L::CODE_SIDE;
+      const uint16_t *ksc = reinterpret_cast<const uint16_t *>(tk + L::OFF_SC);
+      const uint16_t *vsc = reinterpret_cast<const uint16_t *>(tk + L::OFF_SC + L::SC_SIDE);
+      const int tile0 = sp.tile(k) * TP;
+      const bool all = !past && tile0 + TP - 1 <= p_first &&
+                       (a.window <= 0 || tile0 > p_last - a.window || tile0 + TP <= a.sinks);
 
       // scores
-      float sc[MT][2][4];
+      float sc[MP][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mp = 0; mp < MP; ++mp)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[mt][nt][e] = 0.0f;
-#pragma unroll 2
-      for (int gr = 0; gr < C; ++gr) {
-        uint32_t qa[L::PARTS][MT][2][4];
-        float off[MT][2];
+          for (int e = 0; e < 4; ++e) sc[mp][nt][e] = 0.0f;
+      const int r0 = warp * 16 * MP + g8;  // and 8 on, and 16 MP on
+      uint32_t sr[MP][2][C / 2];           // the scales of its rows
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          off[mt][0] = qoff[gr * RB + mt * 16 + g8];
-          off[mt][1] = qoff[gr * RB + mt * 16 + g8 + 8];
+      for (int mp = 0; mp < MP; ++mp)
 #pragma unroll
-          for (int pt = 0; pt < L::PARTS; ++pt)
+        for (int e = 0; e < 2; ++e) {
+          const uint16_t *src = ksc + (r0 + mp * 16 + 8 * e) * chd;
+          if (chd == C) {
+            if constexpr (C == 2) sr[mp][e][0] = *reinterpret_cast<const uint32_t *>(src);
+            else if constexpr (C == 4) *reinterpret_cast<uint2 *>(sr[mp][e]) = *reinterpret_cast<const uint2 *>(src);
+            else {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              const uint4 v = reinterpret_cast<const uint4 *>(sm + pt * L::QF)[((gr * 2 + m) * MT + mt) * 32 + lane];
-              qa[pt][mt][m][0] = v.x, qa[pt][mt][m][1] = v.y, qa[pt][mt][m][2] = v.z, qa[pt][mt][m][3] = v.w;
+              for (int i = 0; i < C / 8; ++i)
+                reinterpret_cast<uint4 *>(sr[mp][e])[i] = reinterpret_cast<const uint4 *>(src)[i];
             }
+          } else {
+#pragma unroll
+            for (int i = 0; i < C / 2; ++i)
+              sr[mp][e][i] = (2 * i < chd ? (uint32_t)src[2 * i] : 0u) |
+                             (2 * i + 1 < chd ? (uint32_t)src[2 * i + 1] << 16 : 0u);
+          }
         }
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const int r = warp * 16 + nt * 8 + g8;
-          const uint32_t w = *reinterpret_cast<const uint32_t *>(tk + r * L::CB + pk_swz<C>(r, gr) * 16 + t4 * 4);
-          const uint32_t w8 = w >> 8;
-          const float2 step = __half22float2(
-              *reinterpret_cast<const __half2 *>(ksc + gr * SCP + warp * 16 + nt * 8 + 2 * t4));
+      for (int gr = 0; gr < C; ++gr) {
+        uint32_t aw[MP][2][4];
+        float st[MP][2];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            float acc[4] = {off[mt][0], off[mt][0], off[mt][1], off[mt][1]};
+        for (int mp = 0; mp < MP; ++mp) {
 #pragma unroll
-            for (int pt = 0; pt < L::PARTS; ++pt) {
-              mma16816(acc, qa[pt][mt][0], w & 0x000f000fu, w & 0x00f000f0u, acc);
-              mma16816(acc, qa[pt][mt][1], w8 & 0x000f000fu, w8 & 0x00f000f0u, acc);
+          for (int e = 0; e < 2; ++e) {
+            const int r = r0 + mp * 16 + 8 * e;
+            const uint8_t *box = tk + ((r >> 6) * L::HALVES + gr / 8) * L::CODE64;
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>(r & 63, gr & 7) + t4 * 4);
+            uint32_t v[4];
+            dequant_i4(w, v);
+            aw[mp][0][e] = v[0];
+            aw[mp][0][2 + e] = v[1];
+            aw[mp][1][e] = v[2];
+            aw[mp][1][2 + e] = v[3];
+            st[mp][e] = __half2float(__ushort_as_half((uint16_t)(sr[mp][e][gr >> 1] >> (16 * (gr & 1)))));
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          uint4 qb[L::PARTS];
+#pragma unroll
+          for (int pt = 0; pt < L::PARTS; ++pt)
+            qb[pt] = reinterpret_cast<const uint4 *>(sm + L::OFF_Q + pt * L::QF)[(gr * NT + nt) * 32 + lane];
+#pragma unroll
+          for (int mp = 0; mp < MP; ++mp) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (SP) {
+              float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma16816(low, aw[mp][0], qb[L::PARTS - 1].x, qb[L::PARTS - 1].y, low);
+              mma16816(low, aw[mp][1], qb[L::PARTS - 1].z, qb[L::PARTS - 1].w, low);
+              mma16816(acc, aw[mp][0], qb[0].x, qb[0].y, acc);
+              mma16816(acc, aw[mp][1], qb[0].z, qb[0].w, acc);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[e] += low[e];
+            } else {
+              mma16816(acc, aw[mp][0], qb[0].x, qb[0].y, acc);
+              mma16816(acc, aw[mp][1], qb[0].z, qb[0].w, acc);
             }
-            sc[mt][nt][0] = fmaf(acc[0], step.x, sc[mt][nt][0]);
-            sc[mt][nt][1] = fmaf(acc[1], step.y, sc[mt][nt][1]);
-            sc[mt][nt][2] = fmaf(acc[2], step.x, sc[mt][nt][2]);
-            sc[mt][nt][3] = fmaf(acc[3], step.y, sc[mt][nt][3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[mp][nt][e] = fmaf(acc[e], st[mp][e >> 1], sc[mp][nt][e]);
           }
         }
       }
 
       // softmax, in powers of two
-      const int tile0 = sp.tile(k) * PACK_TILE, j0 = tile0 + warp * 16 + 2 * t4;
-      const bool all = !past && tile0 + PACK_TILE - 1 <= p_first &&
-                       (a.window <= 0 || tile0 > p_last - a.window || tile0 + PACK_TILE <= a.sinks);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 f = *reinterpret_cast<const float2 *>(fr + nt * 8 + 2 * t4);
+        float mx[2] = {-INFINITY, -INFINITY};
+        if (all) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float f = fr[mt * 16 + g8 + 8 * e];
-          float mx = -INFINITY;
+          for (int mp = 0; mp < MP; ++mp)
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float &x = sc[mt][nt][2 * e + c];
-              const int j = j0 + nt * 8 + c, p = pos[mt][e];
-              const bool see = all || (j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks));
-              x = see ? x * f : -INFINITY;
-              mx = fmaxf(mx, x);
+            for (int e = 0; e < 4; ++e) {
+              sc[mp][nt][e] *= e & 1 ? f.y : f.x;
+              mx[e & 1] = fmaxf(mx[e & 1], sc[mp][nt][e]);
             }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (t4 == 0) wmax[(mt * 16 + g8 + 8 * e) * 4 + warp] = mx;
+        } else {
+#pragma unroll
+          for (int mp = 0; mp < MP; ++mp)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = tile0 + r0 + mp * 16 + 8 * (e >> 1), p = pos[nt][e & 1];
+              const bool see = j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
+              sc[mp][nt][e] = see ? sc[mp][nt][e] * (e & 1 ? f.y : f.x) : -INFINITY;
+              mx[e & 1] = fmaxf(mx[e & 1], sc[mp][nt][e]);
+            }
         }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
+        }
+        if (g8 == 0) {
+          wmax[(nt * 8 + 2 * t4) * 4 + warp] = mx[0];
+          wmax[(nt * 8 + 2 * t4 + 1) * 4 + warp] = mx[1];
+        }
+      }
       __syncthreads();
+      load(k + NS - 1);  // every warp is done with the step before, whose place this takes
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float al[2];
+      for (int nt = 0; nt < NT; ++nt) {
+        float al[2], base[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float4 w4 = *reinterpret_cast<const float4 *>(wmax + (mt * 16 + g8 + 8 * e) * 4);
-          const float mx = fmaxf(fmaxf(fmaxf(w4.x, w4.y), fmaxf(w4.z, w4.w)), m_run[mt][e]);
-          const float base = mx == -INFINITY ? 0.0f : mx;
-          al[e] = exp2_fast(m_run[mt][e] - base);
-          m_run[mt][e] = mx;
-          float sum = 0.0f;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float &x = sc[mt][nt][2 * e + c];
-              x = exp2_fast(x - base + 12.0f);
-              sum += x;
-            }
-          l_run[mt][e] = l_run[mt][e] * al[e] + sum;
+          const float4 w4 = *reinterpret_cast<const float4 *>(wmax + (nt * 8 + 2 * t4 + e) * 4);
+          const float mx = fmaxf(fmaxf(fmaxf(w4.x, w4.y), fmaxf(w4.z, w4.w)), m_run[nt][e]);
+          base[e] = mx == -INFINITY ? 0.0f : mx;
+          al[e] = exp2_fast(m_run[nt][e] - base[e]);
+          m_run[nt][e] = mx;
         }
-        // a warp's scores lie as the weights' fragment of its 16 positions does
-        uint32_t hi[4], lo[4];
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = sc[mt][i >> 1][2 * (i & 1)], y = sc[mt][i >> 1][2 * (i & 1) + 1];
-          hi[i] = half2_bits(x, y);
+        for (int mp = 0; mp < MP; ++mp) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // f32 rows: 2^12 the weight, so that its halves reach 2^-37 of the largest
+            const float x = exp2_fast(sc[mp][nt][e] - base[e & 1]);
+            sc[mp][nt][e] = SP ? x * 4096.0f : x;
+            sum[e & 1] += sc[mp][nt][e];
+          }
+          // the weights turned to the second product's fragment: positions along its depth
+          const uint32_t h0 = half2_bits(sc[mp][nt][0], sc[mp][nt][1]), h1 = half2_bits(sc[mp][nt][2], sc[mp][nt][3]);
+          uint2 *p = reinterpret_cast<uint2 *>(sm + L::OFF_P) + ((warp * MP + mp) * NT + nt) * 32 + lane;
+          *p = make_uint2(transpose8(h0), transpose8(h1));
           if (SP) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-            lo[i] = half2_bits(x - f.x, y - f.y);
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
+            const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+            const uint32_t l0 = half2_bits(sc[mp][nt][0] - f0.x, sc[mp][nt][1] - f0.y);
+            const uint32_t l1 = half2_bits(sc[mp][nt][2] - f1.x, sc[mp][nt][3] - f1.y);
+            p[L::PF / 8] = make_uint2(transpose8(l0), transpose8(l1));
           }
         }
-        reinterpret_cast<uint4 *>(sm + L::OFF_P)[(warp * MT + mt) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (SP)
-          reinterpret_cast<uint4 *>(sm + L::OFF_P + L::PF)[(warp * MT + mt) * 32 + lane] =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        l_run[nt][0] = l_run[nt][0] * al[0] + sum[0];
+        l_run[nt][1] = l_run[nt][1] * al[1] + sum[1];
         if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
 #pragma unroll
-          for (int j = 0; j < NB * 8; ++j) {
-            o[mt][j][0] *= al[0];
-            o[mt][j][1] *= al[0];
-            o[mt][j][2] *= al[1];
-            o[mt][j][3] *= al[1];
-          }
+          for (int j = 0; j < NB * 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][j][e] *= al[e & 1];
         }
       }
       __syncthreads();
 
       // values
+      constexpr int STEPS = TP / 16 / WP;
 #pragma unroll
-      for (int si = 0; si < 4 / WP; ++si) {
-        const int st = wp * (4 / WP) + si;
-        uint32_t pa[L::PARTS][MT][4];
+      for (int si = 0; si < STEPS; ++si) {
+        const int st = wp * STEPS + si;
+        const int r0v = st * 16 + 2 * t4;  // this thread's positions: r0v, + 1, + 8, + 9
+        uint2 pb[L::PARTS][NT];
 #pragma unroll
         for (int pt = 0; pt < L::PARTS; ++pt)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const uint4 v = reinterpret_cast<const uint4 *>(sm + L::OFF_P + pt * L::PF)[(st * MT + mt) * 32 + lane];
-            pa[pt][mt][0] = v.x, pa[pt][mt][1] = v.y, pa[pt][mt][2] = v.z, pa[pt][mt][3] = v.w;
-          }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const int j = (wc * NB + nb) * 2 + (g8 >> 2);  // the 16-byte piece (one group)
-          uint32_t w[4];
-          __half2 step[2];
+          for (int nt = 0; nt < NT; ++nt)
+            pb[pt][nt] = reinterpret_cast<const uint2 *>(sm + L::OFF_P + pt * L::PF)[(st * NT + nt) * 32 + lane];
+        uint32_t live[2] = {0xffffffffu, 0xffffffffu};  // positions no row sees count as 0 whatever lies there
+        if (!all) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int r = st * 16 + 8 * i + 2 * t4;
-            const uint8_t *row = tv + r * L::CB + (g8 & 3) * 4;
-            w[2 * i] = *reinterpret_cast<const uint32_t *>(row + pk_swz<C>(r, j) * 16);
-            w[2 * i + 1] = *reinterpret_cast<const uint32_t *>(row + L::CB + pk_swz<C>(r + 1, j) * 16);
-            step[i] = *reinterpret_cast<const __half2 *>(vsc + j * SCP + r);
+            const int p = tile0 + r0v + 8 * i;
+            const bool x = p < sp.hi && (p >= sp.lo || p < a.sinks);
+            const bool y = p + 1 < sp.hi && (p + 1 >= sp.lo || p + 1 < a.sinks);
+            live[i] = (x ? 0xffffu : 0u) | (y ? 0xffff0000u : 0u);
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int cb = wc * NB + nb;  // 64 columns: groups 2 cb, 2 cb + 1
+          uint32_t rows2[4];            // their scales at each position
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint16_t *src = vsc + (r0v + (i & 1) + 8 * (i >> 1)) * chd + 2 * cb;
+            if ((chd & 1) == 0) {
+              rows2[i] = 2 * cb < chd ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+            } else {
+              rows2[i] = (2 * cb < chd ? (uint32_t)src[0] : 0u) | (2 * cb + 1 < chd ? (uint32_t)src[1] << 16 : 0u);
+            }
           }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {  // columns 0-3, then 4-7 of the thread's eight
-            uint32_t v[2][4];  // [positions 2t.., 2t + 8..][column]
+          for (int gi = 0; gi < 2; ++gi) {
+            uint32_t step[2], x[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              dequant_i4(__byte_perm(w[2 * i], w[2 * i + 1], hf ? 0x7632 : 0x5410), v[i]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t vh[2], vl[2];
+            for (int i = 0; i < 2; ++i) {
+              step[i] = __byte_perm(rows2[2 * i], rows2[2 * i + 1], gi ? 0x7632 : 0x5410) & live[i];
+              const int r = r0v + 8 * i;
+              const uint8_t *box = tv + ((r >> 6) * L::HALVES + cb / 4) * L::CODE64 + (g8 >> 1) * 4;
+              const int j = (cb & 3) * 2 + gi;
+              const uint32_t w0 = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>(r & 63, j));
+              const uint32_t w1 = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>((r & 63) + 1, j));
+              x[i] = __byte_perm(w0, w1, g8 & 1 ? 0x7632 : 0x5410);
+            }
+            // product u: columns 2u (rows 0-7) and 2u + 1 (rows 8-15) of the thread's four
+            uint32_t av[2][4], al[2][4];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const __half2 n2 = *reinterpret_cast<const __half2 *>(&v[i][c]);
-                const __half2 x = __hmul2(n2, step[i]);
-                vh[i] = *reinterpret_cast<const uint32_t *>(&x);
-                if (SP) {
-                  const __half2 y = __hfma2(n2, step[i], __hneg2(x));
-                  vl[i] = *reinterpret_cast<const uint32_t *>(&y);
-                }
-              }
+                uint32_t v[4];
+                dequant_i4(x[i], v);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                float(&acc)[4] = o[mt][nb * 8 + hf * 4 + c];
-                mma16816(acc, pa[0][mt], vh[0], vh[1], acc);
-                if (SP) {
-                  mma16816(acc, pa[1][mt], vh[0], vh[1], acc);
-                  mma16816(acc, pa[0][mt], vl[0], vl[1], acc);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const uint32_t c = v[2 * u + e];
+                    if (SP) {
+                      const uint32_t hi = mul2(c, step[i]);
+                      av[u][2 * i + e] = hi;
+                      al[u][2 * i + e] = rest2(c, step[i], hi);
+                    } else {
+                      av[u][2 * i + e] = c;
+                    }
+                  }
+              }
+            if (!SP) {
+              step[0] = mul2(step[0], 0x48004800u);  // 8: weights of small scales stay above f16's smallest
+              step[1] = mul2(step[1], 0x48004800u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (SP) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                  mma16816(acc, al[u], pb[0][nt].x, pb[0][nt].y, acc);
+                  mma16816(acc, av[u], pb[L::PARTS - 1][nt].x, pb[L::PARTS - 1][nt].y, acc);
+                  mma16816(acc, av[u], pb[0][nt].x, pb[0][nt].y, acc);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[nt][nb * 4 + gi * 2 + u][e] += acc[e];
                 }
+              } else {
+                const uint32_t b0 = mul2(pb[0][nt].x, step[0]), b1 = mul2(pb[0][nt].y, step[1]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) mma16816(o[nt][nb * 4 + gi * 2 + u], av[u], b0, b1, o[nt][nb * 4 + gi * 2 + u]);
               }
             }
           }
         }
       }
     }
-    cp_wait<0>();
+    step0 += kb - ka;
+    if (!SP) {  // undo the 8 the weights carried
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < NB * 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][j][e] *= 0.125f;
+    }
 
     // ---- the rows' sums, and of a narrow head the warps' shares, joined
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float l = l_run[mt][e];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t4 == 0) wsum[(mt * 16 + g8 + 8 * e) * 4 + warp] = l;
+        float l = l_run[nt][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        if (g8 == 0) wsum[(nt * 8 + 2 * t4 + e) * 4 + warp] = l;
       }
     __syncthreads();
     if (WP > 1) {
-      float *buf = reinterpret_cast<float *>(sm + L::OFF_CODE);
+      float *buf = reinterpret_cast<float *>(sm);
       for (int r = 1; r < WP; ++r) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < NB * 8; ++j)
+          for (int j = 0; j < NB * 4; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float *x = buf + (((mt * WC + wc) * NB * 8 + j) * 4 + e) * 32 + lane;
-              if (wp == r) *x = o[mt][j][e];
+              float *x = buf + (((nt * WC + wc) * NB * 4 + j) * 4 + e) * 32 + lane;
+              if (wp == r) *x = o[nt][j][e];
             }
         __syncthreads();
         if (wp == 0) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < NB * 8; ++j)
+            for (int j = 0; j < NB * 4; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[mt][j][e] += buf[(((mt * WC + wc) * NB * 8 + j) * 4 + e) * 32 + lane];
+              for (int e = 0; e < 4; ++e) o[nt][j][e] += buf[(((nt * WC + wc) * NB * 4 + j) * 4 + e) * 32 + lane];
         }
         __syncthreads();
       }
+      fence_async_smem();  // the ring's next copies come after these reads
     }
     if (wp == 0) {
       const bool wide = wide_rows(a.out);
       float *pw = a.work + place * ((size_t)RB * (size + 2));
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = mt * 16 + g8 + 8 * e, rr = b * RB + r;
+          const int r = nt * 8 + 2 * t4 + e, rr = b * RB + r;
           if (rr >= q.n * group) continue;
           const float4 l4 = *reinterpret_cast<const float4 *>(wsum + r * 4);
           const float l = l4.x + l4.y + l4.z + l4.w;
           const float inv = whole ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
+          const size_t to = (size_t)(q.first + rr / group) * a.out.row_stride +
+                            (size_t)(h * group + rr % group) * a.out.head_stride;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = (wc * NB + nb) * 64 + 16 * t4 + 8 * c;
-              if (col >= size) continue;
-              float x[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = o[mt][nb * 8 + j][2 * e + c] * inv;
-              if (whole) {
-                store8(a.out.data, a.out.type,
-                       (size_t)(q.first + rr / group) * a.out.row_stride +
-                           (size_t)(h * group + rr % group) * a.out.head_stride + col,
-                       wide, x);
-              } else {
-                store8(pw, 1, (size_t)r * size + col, (size & 3) == 0, x);
-              }
-            }
-          if (!whole && wc == 0 && t4 == 0) {
-            pw[(size_t)RB * size + r] = m_run[mt][e];
+          for (int j = 0; j < NB * 2; ++j) {  // a group's four columns
+            const int col = (wc * NB * 2 + j) * 32 + 4 * g8;
+            if (col >= size) continue;
+            const float x[4] = {o[nt][2 * j][e] * inv, o[nt][2 * j][2 + e] * inv, o[nt][2 * j + 1][e] * inv,
+                                o[nt][2 * j + 1][2 + e] * inv};
+            if (whole) store4(a.out.data, a.out.type, to + col, wide, x);
+            else *reinterpret_cast<float4 *>(pw + (size_t)r * size + col) = make_float4(x[0], x[1], x[2], x[3]);
+          }
+          if (!whole && wc == 0 && g8 == 0) {
+            pw[(size_t)RB * size + r] = m_run[nt][e];
             pw[(size_t)RB * size + RB + r] = l;
           }
         }
     }
 
     // ---- the next unit
-    if (!spread) return;
+    if (!spread) break;
     at += kb - ka;
-    if (at >= end) return;
+    if (at >= end) break;
     part = 0;
+    bool more = true;
     do {
       if (++h == a.c.heads) {
         h = 0;
         ++b;
-        while (b >= blocks_of(a, q, RB)) {
+        while (more && b >= blocks_of(a, q, RB)) {
           b = 0;
-          if (++s >= a.r.count) return;
-          q = seq_at(a.c, a.r, s);
+          if (++s >= a.r.count) more = false;
+          else q = seq_at(a.c, a.r, s);
         }
       }
-    } while (block_span(a, q, b, RB).count() == 0);
+    } while (more && block_span(a, q, b, RB, TP).count() == 0);
+    if (!more) break;
   }
+  if (gave_up) pack_trouble(a.c);
 }
 
 // ---------------------------------------------------------------------------
-// the pieces of a unit joined, and rows that see nothing set to zero: a warp a
-// row, pieces in order
+// the pieces of a unit joined, and rows that see nothing set to zero: a block
+// a row, its threads four columns each and, of narrow heads, every second or
+// fourth (eighth) piece; each column's pieces are added in a fixed order
 
 struct PackMerge {
   PackAttend a;
-  int rb, spread, parts, grid, blocks;
+  int rb, tp, spread, parts, grid, blocks;
 };
 
-__global__ void __launch_bounds__(128) pack_merge_kernel(PackMerge g) {
+constexpr int PM_THREADS = 128, PM_CHUNK = 256;  // pieces whose factors are kept at a time
+
+__global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(PackMerge g) {
   __shared__ int red[16];
+  __shared__ float pm[PM_CHUNK], pl[PM_CHUNK];
+  __shared__ float4 part4[PM_THREADS];
   const PackAttend &a = g.a;
-  const int RB = g.rb, size = a.c.size;
-  pdl_wait();
-  pdl_release();
+  const int RB = g.rb, TP = g.tp, size = a.c.size, tid = threadIdx.x;
   int u = blockIdx.x, s, b, h = u % a.c.heads, first, last, share = 0, n;
   SeqAt q;
   u /= a.c.heads;
+  const int r = blockIdx.y;
   if (g.spread) {
     s = u / g.blocks;
     b = u - s * g.blocks;
-    int before;
-    const int total = list_total(a, RB, true, s, &before, red);
-    share = share_of(total, g.grid);
     q = seq_at(a.c, a.r, s);
-    if (b >= blocks_of(a, q, RB)) return;
-    for (int i = 0; i < b; ++i) before += block_span(a, q, i, RB).count() * a.c.heads;
-    n = block_span(a, q, b, RB).count();
+    if (b * RB + r >= q.n * a.group) return;
+    int before;
+    const int total = list_total(a, RB, TP, true, s, &before, red);
+    share = share_of(total, g.grid);
+    for (int i = 0; i < b; ++i) before += block_span(a, q, i, RB, TP).count() * a.c.heads;
+    n = block_span(a, q, b, RB, TP).count();
     before += h * n;
     first = before / share;
     last = (before + max(n, 1) - 1) / share;
     if (n > 0 && first == last) return;  // one block had it all
     u = before;
   } else {
-    const int total = list_total(a, RB, false, 0, nullptr, red);
+    const int total = list_total(a, RB, TP, false, 0, nullptr, red);
     if (u >= total) return;
-    const ListAt f = list_at(a, RB, false, total - 1 - u, red);
+    const ListAt f = list_at(a, RB, TP, false, total - 1 - u, red);
     s = f.s;
     if (s < 0) return;
     b = total - 1 - u - f.before;
     q = seq_at(a.c, a.r, s);
-    n = block_span(a, q, b, RB).count();
+    if (b * RB + r >= q.n * a.group) return;
+    n = block_span(a, q, b, RB, TP).count();
     first = 0;
     last = g.parts - 1;
     u = blockIdx.x * g.parts;
   }
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, rr = b * RB + r;
-  if (rr >= q.n * a.group) return;
+  const int rr = b * RB + r;
   const size_t piece = (size_t)RB * (size + 2);
+  auto place = [&](int i) {
+    return g.spread ? 2 * (size_t)i + (i * share <= u ? 1 : 0)  // the piece with the unit's first tile
+                    : (size_t)u + i;
+  };
+  const int lanes = size / 4, teams = PM_THREADS / lanes, team = tid / lanes, col = 4 * (tid - team * lanes);
   float m = -INFINITY, l = 0.0f;
-  float x[2][8] = {};
-  if (n > 0) {
-    for (int i = first; i <= last; ++i) {
-      size_t place;
-      if (g.spread) {
-        place = 2 * (size_t)i + (i * share <= u ? 1 : 0);  // the piece with the unit's first tile
-      } else {
-        if ((long)n * i / g.parts == (long)n * (i + 1) / g.parts) continue;
-        place = (size_t)u + i;
-      }
-      const float *pw = a.work + place * piece;
-      const float pm = pw[(size_t)RB * size + r], pl = pw[(size_t)RB * size + RB + r];
-      if (pl == 0.0f) continue;  // it saw none of the row's positions
-      const float mx = fmaxf(m, pm), f0 = exp2_fast(m - mx), f1 = exp2_fast(pm - mx);
-      m = mx;
-      l = l * f0 + pl * f1;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = lane * 8 + e * 256;
-        if (col >= size) continue;
-        float y[8];
-        load8(pw, 1, (size_t)r * size + col, true, y);
-#pragma unroll
-        for (int i2 = 0; i2 < 8; ++i2) x[e][i2] = x[e][i2] * f0 + y[i2] * f1;
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  pdl_wait();
+  for (int c0 = first; n > 0 && c0 <= last; c0 += PM_CHUNK) {
+    const int cn = min(PM_CHUNK, last + 1 - c0);
+    float mx = m;
+    __syncthreads();
+    for (int i = tid; i < cn; i += PM_THREADS) {
+      const int p = c0 + i;
+      const bool none = !g.spread && (long)n * p / g.parts == (long)n * (p + 1) / g.parts;
+      const float *pw = a.work + place(p) * piece + (size_t)RB * size + r;
+      const float y = none ? 0.0f : pw[RB];
+      pl[i] = y;
+      pm[i] = y == 0.0f ? -INFINITY : pw[0];  // a piece that saw none of the row's positions
+    }
+    __syncthreads();
+    for (int i = 0; i < cn; ++i) mx = fmaxf(mx, pm[i]);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    const float back = exp2_fast(m - base);
+    m = mx;
+    l *= back;
+    x.x *= back, x.y *= back, x.z *= back, x.w *= back;
+    for (int i = 0; i < cn; ++i) {
+      const float y = pl[i];
+      if (y != 0.0f) l += y * exp2_fast(pm[i] - base);
+    }
+    if (team < teams) {
+#pragma unroll 4
+      for (int i = team; i < cn; i += teams) {
+        if (pl[i] == 0.0f) continue;
+        const float f = exp2_fast(pm[i] - base);
+        const float4 y = *reinterpret_cast<const float4 *>(a.work + place(c0 + i) * piece + (size_t)r * size + col);
+        x.x = fmaf(y.x, f, x.x);
+        x.y = fmaf(y.y, f, x.y);
+        x.z = fmaf(y.z, f, x.z);
+        x.w = fmaf(y.w, f, x.w);
       }
     }
   }
-  const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
-  if (n == 0 && lane == 0 && (q.slot < 0 || q.fill + rr / a.group >= a.c.positions)) pack_trouble(a.c);
-  const bool wide = wide_rows(a.out);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int col = lane * 8 + e * 256;
-    if (col >= size) continue;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[e][i] *= inv;
-    store8(a.out.data, a.out.type,
-           (size_t)(q.first + rr / a.group) * a.out.row_stride +
-               (size_t)(h * a.group + rr % a.group) * a.out.head_stride + col,
-           wide, x[e]);
+  part4[tid] = x;
+  __syncthreads();
+  if (n == 0 && tid == 0 && (q.slot < 0 || q.fill + rr / a.group >= a.c.positions)) pack_trouble(a.c);
+  if (team != 0) return;
+  for (int i = 1; i < teams; ++i) {
+    const float4 y = part4[i * lanes + tid];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
   }
+  const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
+  const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+  store4(a.out.data, a.out.type,
+         (size_t)(q.first + rr / a.group) * a.out.row_stride +
+             (size_t)(h * a.group + rr % a.group) * a.out.head_stride + col,
+         wide_rows(a.out), y);
 }
 
 template <typename... P, typename... Q>
@@ -1061,15 +1204,17 @@ cudaError_t pack_launch(void (*kern)(P...), dim3 grid, int threads, size_t smem,
 // its shared memory allowed and how many blocks an SM holds.
 constexpr int PACK_DEVICES = 64;
 
-template <int HDP, int MT, bool SP>
-cudaError_t pack_form_ready(int *per_sm) {
+template <int HDP, int NT, bool SP>
+cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
+  using L = PackTile<HDP, NT, SP>;
+  plan->tile = L::TP;
+  plan->pitch = L::PITCH;
   static std::atomic<int> known[PACK_DEVICES];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < PACK_DEVICES && (*per_sm = known[dev].load()) > 0) return cudaSuccess;
-  auto kern = pack_attend_kernel<HDP, MT, SP>;
-  using L = PackTile<HDP, MT, SP>;
+  auto kern = pack_attend_kernel<HDP, NT, SP>;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kern, 128, L::SMEM);
   if (e == cudaSuccess && *per_sm < 1) e = cudaErrorInvalidConfiguration;
@@ -1077,39 +1222,49 @@ cudaError_t pack_form_ready(int *per_sm) {
   return e;
 }
 
-template <int HDP, int MT, bool SP>
-cudaError_t pack_form_launch(const PackAttend &a, const PackPlan &p, cudaStream_t st) {
-  return pack_launch(pack_attend_kernel<HDP, MT, SP>, dim3(p.grid), 128, PackTile<HDP, MT, SP>::SMEM, st, false, a,
-                     p.spread, p.parts);
+template <int HDP, int NT, bool SP>
+cudaError_t pack_form_launch(const PackAttend &a, const PackPlan &p, const CUtensorMap &tmk, const CUtensorMap &tmv,
+                             cudaStream_t st) {
+  return pack_launch(pack_attend_kernel<HDP, NT, SP>, dim3(p.grid), 128, PackTile<HDP, NT, SP>::SMEM, st, false, a,
+                     tmk, tmv, p.spread, p.parts);
 }
 
 // Calls F for the form a plan names.
-#define PACK_FORMS(F, p, ...)                                                                      \
-  switch ((p).wide * 8 + (p).tiles16 * 2 + (p).split2) {                                          \
-    case 64 * 8 + 2: return F<64, 1, false>(__VA_ARGS__);                                          \
-    case 64 * 8 + 4: return F<64, 2, false>(__VA_ARGS__);                                          \
-    case 64 * 8 + 8: return F<64, 4, false>(__VA_ARGS__);                                          \
-    case 64 * 8 + 3: return F<64, 1, true>(__VA_ARGS__);                                           \
-    case 64 * 8 + 5: return F<64, 2, true>(__VA_ARGS__);                                           \
-    case 128 * 8 + 2: return F<128, 1, false>(__VA_ARGS__);                                        \
-    case 128 * 8 + 4: return F<128, 2, false>(__VA_ARGS__);                                        \
-    case 128 * 8 + 8: return F<128, 4, false>(__VA_ARGS__);                                        \
-    case 128 * 8 + 3: return F<128, 1, true>(__VA_ARGS__);                                         \
-    case 128 * 8 + 5: return F<128, 2, true>(__VA_ARGS__);                                         \
-    case 256 * 8 + 2: return F<256, 1, false>(__VA_ARGS__);                                        \
-    case 256 * 8 + 4: return F<256, 2, false>(__VA_ARGS__);                                        \
-    case 256 * 8 + 8: return F<256, 4, false>(__VA_ARGS__);                                        \
-    case 256 * 8 + 3: return F<256, 1, true>(__VA_ARGS__);                                         \
-    case 256 * 8 + 5: return F<256, 2, true>(__VA_ARGS__);                                         \
-    case 512 * 8 + 2: return F<512, 1, false>(__VA_ARGS__);                                        \
-    case 512 * 8 + 4: return F<512, 2, false>(__VA_ARGS__);                                        \
-    case 512 * 8 + 3: return F<512, 1, true>(__VA_ARGS__);                                         \
-    default: return cudaErrorInvalidValue;                                                        \
+#define PACK_FORMS(F, p, ...)                     \
+  switch ((p).wide * 16 + (p).rows8 * 2 + (p).split2) { \
+    case 1024 + 2 + 0: return F<64, 1, false>(__VA_ARGS__); \
+    case 1024 + 4 + 0: return F<64, 2, false>(__VA_ARGS__); \
+    case 1024 + 8 + 0: return F<64, 4, false>(__VA_ARGS__); \
+    case 1024 + 16 + 0: return F<64, 8, false>(__VA_ARGS__); \
+    case 1024 + 2 + 1: return F<64, 1, true>(__VA_ARGS__); \
+    case 1024 + 4 + 1: return F<64, 2, true>(__VA_ARGS__); \
+    case 1024 + 8 + 1: return F<64, 4, true>(__VA_ARGS__); \
+    case 2048 + 2 + 0: return F<128, 1, false>(__VA_ARGS__); \
+    case 2048 + 4 + 0: return F<128, 2, false>(__VA_ARGS__); \
+    case 2048 + 8 + 0: return F<128, 4, false>(__VA_ARGS__); \
+    case 2048 + 16 + 0: return F<128, 8, false>(__VA_ARGS__); \
+    case 2048 + 2 + 1: return F<128, 1, true>(__VA_ARGS__); \
+    case 2048 + 4 + 1: return F<128, 2, true>(__VA_ARGS__); \
+    case 2048 + 8 + 1: return F<128, 4, true>(__VA_ARGS__); \
+    case 4096 + 2 + 0: return F<256, 1, false>(__VA_ARGS__); \
+    case 4096 + 4 + 0: return F<256, 2, false>(__VA_ARGS__); \
+    case 4096 + 8 + 0: return F<256, 4, false>(__VA_ARGS__); \
+    case 4096 + 16 + 0: return F<256, 8, false>(__VA_ARGS__); \
+    case 4096 + 2 + 1: return F<256, 1, true>(__VA_ARGS__); \
+    case 4096 + 4 + 1: return F<256, 2, true>(__VA_ARGS__); \
+    case 4096 + 8 + 1: return F<256, 4, true>(__VA_ARGS__); \
+    case 8192 + 2 + 0: return F<512, 1, false>(__VA_ARGS__); \
+    case 8192 + 4 + 0: return F<512, 2, false>(__VA_ARGS__); \
+    case 8192 + 8 + 0: return F<512, 4, false>(__VA_ARGS__); \
+    case 8192 + 2 + 1: return F<512, 1, true>(__VA_ARGS__); \
+    case 8192 + 4 + 1: return F<512, 2, true>(__VA_ARGS__); \
+    default: return cudaErrorInvalidValue;        \
   }
 
-static cudaError_t pack_form(const PackPlan &p, int *per_sm) { PACK_FORMS(pack_form_ready, p, per_sm) }
-static cudaError_t pack_run(const PackPlan &p, const PackAttend &a, cudaStream_t st) {
-  PACK_FORMS(pack_form_launch, p, a, p, st)
+static cudaError_t pack_form(PackPlan *p, int *per_sm) { PACK_FORMS(pack_form_ready, *p, p, per_sm) }
+static cudaError_t pack_run(const PackPlan &p, const PackAttend &a, const CUtensorMap &tmk, const CUtensorMap &tmv,
+                            cudaStream_t st) {
+  PACK_FORMS(pack_form_launch, p, a, p, tmk, tmv, st)
 }
 
 static cudaError_t pack_sms(int *sms) {
@@ -1153,19 +1308,20 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   p->wide = size <= 64 ? 64 : size <= 128 ? 128 : size <= 256 ? 256 : 512;
   p->split2 = type == 1 ? 1 : 0;
   const long need = (long)rows_most * group;
-  const int most16 = p->wide == 512 ? (p->split2 ? 1 : 2) : (p->split2 ? 2 : 4);
-  p->tiles16 = need <= 16 ? 1 : need <= 32 || most16 < 4 ? 2 : 4;
-  if (p->tiles16 > most16) p->tiles16 = most16;
-  const int rb = 16 * p->tiles16;
+  int most8 = p->split2 ? 4 : 8;  // what registers hold
+  if (p->wide == 512) most8 /= 2;
+  p->rows8 = need <= 8 ? 1 : need <= 16 ? 2 : need <= 32 ? 4 : 8;
+  if (p->rows8 > most8) p->rows8 = most8;
+  const int rb = 8 * p->rows8;
   int sms = 0, per_sm = 0;
   cudaError_t e = pack_sms(&sms);
-  if (e == cudaSuccess) e = pack_form(*p, &per_sm);
+  if (e == cudaSuccess) e = pack_form(p, &per_sm);
   if (e != cudaSuccess) return e;
   const long blocks = (need + rb - 1) / rb;
   const long slots = (long)sms * per_sm;
   // the most tiles a unit can have: its rows' reach, wherever it starts in a tile
-  const long reach = window > 0 ? (long)window + rb / group + 1 + sinks + 3 * PACK_TILE : positions;
-  const long tiles = ((reach < positions ? reach : positions) + PACK_TILE - 1) / PACK_TILE;
+  const long reach = window > 0 ? (long)window + rb / group + 1 + sinks + 3 * p->tile : positions;
+  const long tiles = ((reach < positions ? reach : positions) + p->tile - 1) / p->tile;
   p->spread = blocks <= 8;
   long grid;
   if (p->spread) {
@@ -1190,11 +1346,43 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   return cudaSuccess;
 }
 
+// The tensor map of one side's codes: [slot, head, position][size / 2] bytes
+// in boxes of 64 positions by `pitch` bytes, swizzled over the pitch; columns
+// past the head arrive as zeros.  Host only.
+static cudaError_t pack_map(const PackView &c, const void *codes, int pitch, CUtensorMap *map) {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+  PFN_cuTensorMapEncodeTiled_v12000 encode = known.load();
+  if (!encode) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (found != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    known.store(encode);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)c.size / 2, (cuuint64_t)c.slots * c.heads * c.positions};
+  const cuuint64_t strides[1] = {(cuuint64_t)c.size / 2};
+  const cuuint32_t box[2] = {(cuuint32_t)pitch, 64}, step[2] = {1, 1};
+  const CUtensorMapSwizzle swz = pitch == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : pitch == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                               : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 cudaError_t igc_launch_pack_attend(const PackAttend *a, const PackPlan *p, cudaStream_t st, int *launches) {
+  *launches = 0;
+  CUtensorMap tmk, tmv;
+  cudaError_t e = pack_map(a->c, a->c.kc, p->pitch, &tmk);
+  if (e == cudaSuccess) e = pack_map(a->c, a->c.vc, p->pitch, &tmv);
+  if (e != cudaSuccess) return e;
   *launches = 1;
-  cudaError_t e = pack_run(*p, *a, st);
+  e = pack_run(*p, *a, tmk, tmv, st);
   if (e != cudaSuccess || (!p->spread && p->parts == 1)) return e;
   *launches = 2;
-  const PackMerge g = {*a, 16 * p->tiles16, p->spread, p->parts, p->grid, p->blocks};
-  return pack_launch(pack_merge_kernel, dim3((unsigned)p->units, 4 * p->tiles16), 128, 0, st, true, g);
+  const PackMerge g = {*a, 8 * p->rows8, p->tile, p->spread, p->parts, p->grid, p->blocks};
+  return pack_launch(pack_merge_kernel, dim3((unsigned)p->units, 8 * p->rows8), PM_THREADS, 0, st, true, g);
 }

@@ -46,9 +46,11 @@ struct PackAttend {
 
 // How a call's attention runs, from its host-known sizes alone.
 struct PackPlan {
-  int tiles16;   // 16-row tiles a block holds (1, 2 or 4)
+  int rows8;     // eights of query rows a block holds (1, 2, 4 or 8)
   int wide;      // head width the kernel is built for: 64, 128, 256 or 512
   int split2;    // f32 rows: hi and lo halves of both operands
+  int tile;      // positions a step
+  int pitch;     // code bytes of a row of a TMA box
   int blocks;    // blocks a sequence can need, at most
   int spread;    // 1: one list of tiles over all units, an equal share a block; 0: `parts` blocks a unit
   int parts;

@@ -3308,7 +3308,8 @@ bool pack_sane(const igc_pack *p) {
   if (p->slot_count < 1 || p->head_count < 1 || p->position_count < PACK_TILE || p->position_count % PACK_TILE != 0)
     return false;
   if (p->head_size < PACK_GROUP || p->head_size > 512 || p->head_size % PACK_GROUP != 0) return false;
-  return p->device >= 0 && p->position_count <= (1 << 30) && p->head_count <= (1 << 16);
+  if (p->device < 0 || p->head_count > (1 << 16)) return false;
+  return (double)p->slot_count * p->head_count * p->position_count < 2147483648.0;  // positions are counted in ints
 }
 
 bool pack_rows_sane(const igc_pack *p, const igc_pack_rows *r) {

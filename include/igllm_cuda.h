@@ -352,7 +352,8 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * is stored as 0.  Codes are [slot][head][position][head_size / 2] bytes,
  * scales [slot][head][position][head_size / 32] halves, keys and values apart,
  * each array on a 16-byte boundary; `position_count` is a multiple of 64 and
- * `head_size` of 32, at most 512.  `trouble`, when not NULL, is a device word
+ * `head_size` of 32, at most 512; slots, heads and positions multiply to less
+ * than 2^31.  `trouble`, when not NULL, is a device word
  * (zero at first) that calls set where what they find on the device does not
  * fit the cache; igc_pack_status reads and clears it.
  *
