@@ -311,7 +311,7 @@ struct PackTile {
   static constexpr int HALVES = HDP / 2 / PITCH;         // rows of 512 columns lie in two halves
   static constexpr int MP = NT <= 2 && HDP <= 256 ? 2 : 1;
   static constexpr int TP = 64 * MP;                     // positions a step
-  static constexpr int NS = HDP <= 128 ? 3 : MP == 2 || HDP == 512 ? 2 : 3;  // steps in flight
+  static constexpr int NS = MP == 2 || HDP == 512 ? 2 : 3;  // steps in flight
   static constexpr int WC = HDP >= 256 ? 4 : HDP / 64;   // warps across the columns
   static constexpr int WP = 4 / WC;                      // warps across a step's positions
   static constexpr int NB = HDP / 64 / WC;               // 64-column blocks a warp
@@ -333,7 +333,7 @@ struct PackTile {
   static constexpr int OFF_P = OFF_SUM + 4 * RB * 4;
   static constexpr int SMEM = 1024 + OFF_P + PF * PARTS;
   // blocks an SM that registers are kept for
-  static constexpr int PER_SM = NT == 1 ? (HDP <= 128 ? 4 : 3) : NT == 2 && HDP <= 256 ? 3 : 2;
+  static constexpr int PER_SM = NT == 1 ? (HDP <= 128 ? 4 : 3) : NT <= 4 && HDP <= 256 ? 3 : 2;
 };
 
 // Where the 16-byte piece j of position row r lies in a box of PITCH-byte
@@ -352,6 +352,13 @@ __device__ __forceinline__ void pk_load(void *dst, const CUtensorMap *map, int x
           smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
+}
+
+// mma16816 of igc_device.cuh, free to be scheduled: d += a b.
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -404,7 +411,7 @@ __device__ __forceinline__ TileSpan span_of(const PackAttend &a, const SeqAt &q,
 
 // Block b (of RB rows) of a sequence: its tokens.
 __device__ __forceinline__ TileSpan block_span(const PackAttend &a, const SeqAt &q, int b, int rb, int tp) {
-  const int t0 = b * rb / a.group, t1 = min(q.n - 1, ((b + 1) * rb - 1) / a.group);
+  const int t0 = a.by_group.of(b * rb), t1 = min(q.n - 1, a.by_group.of((b + 1) * rb - 1));
   return span_of(a, q, t0, t1, tp);
 }
 
@@ -414,6 +421,7 @@ __device__ __forceinline__ int blocks_of(const PackAttend &a, const SeqAt &q, in
 
 // Sums over the block (every thread gets the total); `red` holds a word a
 // warp and two more.
+constexpr int PACK_WARPS = 16;  // the most of any block
 __device__ __forceinline__ int block_total(int v, int *red) {
   v = __reduce_add_sync(0xffffffffu, v);
   __syncthreads();
@@ -464,7 +472,7 @@ struct ListAt {
 };
 __device__ __forceinline__ ListAt list_at(const PackAttend &a, int rb, int tp, bool spread, int want, int *red) {
   ListAt at = {0, -1, 0};
-  int *found = red + 8;
+  int *found = red + PACK_WARPS;
   if (threadIdx.x == 0) found[0] = -1;
   for (int base = 0; base < a.r.count; base += blockDim.x) {
     int t;
@@ -507,7 +515,7 @@ __device__ __forceinline__ int share_of(int total, int grid) {
 __device__ __forceinline__ int list_share(const PackAttend &a, int rb, int tp, int grid, int mine, ListAt *at,
                                           int *red) {
   if (a.r.count <= (int)blockDim.x) {
-    int *found = red + 8;
+    int *found = red + PACK_WARPS;
     if (threadIdx.x == 0) found[0] = -1;
     const int w = seq_weight(a, threadIdx.x, rb, tp, true);
     const int before = block_scan(w, red, &at->total);
@@ -527,7 +535,93 @@ __device__ __forceinline__ int list_share(const PackAttend &a, int rb, int tp, i
   return share;
 }
 
-template <int HDP, int NT, bool SP>
+// The units of a block's share, in the order every warp walks them.
+struct PackWalk {
+  int at, end, s, b, h, part, n, ka, kb;
+  bool whole;
+  size_t place;
+  SeqAt q;
+  TileSpan sp;
+};
+
+// The block's first unit; false where it has none.
+template <int RB, int TP>
+__device__ __forceinline__ bool walk_start(const PackAttend &a, int spread, int parts, PackWalk &w, int *red) {
+  w.at = w.end = w.h = w.b = w.part = 0;
+  if (spread) {
+    ListAt f;
+    const int share = list_share(a, RB, TP, gridDim.x, blockIdx.x, &f, red);
+    w.at = blockIdx.x * share;
+    w.end = min(f.total, w.at + share);
+    if (w.at >= w.end || f.s < 0) return false;
+    w.s = f.s;
+    w.q = seq_at(a.c, a.r, w.s);
+    int left = w.at - f.before;
+    for (;; ++w.b) {
+      if (w.b >= blocks_of(a, w.q, RB)) return false;
+      const int n = block_span(a, w.q, w.b, RB, TP).count() * a.c.heads;
+      if (left < n) {
+        w.h = left / (n / a.c.heads);
+        w.part = left - w.h * (n / a.c.heads);  // the step of the unit it starts at
+        return true;
+      }
+      left -= n;
+    }
+  }
+  const int u = blockIdx.x / parts;
+  w.part = blockIdx.x - u * parts;
+  w.h = u % a.c.heads;
+  const int total = list_total(a, RB, TP, false, 0, nullptr, red);
+  const int vb = total - 1 - u / a.c.heads;  // the rows at the end see the most: first
+  if (vb < 0) return false;
+  const ListAt f = list_at(a, RB, TP, false, vb, red);
+  w.s = f.s;
+  if (w.s < 0) return false;
+  w.b = vb - f.before;
+  w.q = seq_at(a.c, a.r, w.s);
+  return true;
+}
+
+// The steps [ka, kb) of the unit that are this block's.
+template <int RB, int TP>
+__device__ __forceinline__ void walk_unit(const PackAttend &a, int spread, int parts, PackWalk &w) {
+  w.sp = block_span(a, w.q, w.b, RB, TP);
+  w.n = w.sp.count();
+  if (spread) {
+    w.ka = w.part;
+    w.kb = min(w.n, w.part + (w.end - w.at));
+    w.whole = w.ka == 0 && w.kb == w.n;
+    w.place = 2 * (size_t)blockIdx.x + (w.ka == 0 ? 1 : 0);
+  } else {
+    w.ka = (int)((long)w.n * w.part / parts);
+    w.kb = (int)((long)w.n * (w.part + 1) / parts);
+    w.whole = parts == 1;
+    w.place = blockIdx.x;
+  }
+}
+
+// On to the next unit; false at the end.
+template <int RB, int TP>
+__device__ __forceinline__ bool walk_next(const PackAttend &a, int spread, PackWalk &w) {
+  if (!spread) return false;
+  w.at += w.kb - w.ka;
+  if (w.at >= w.end) return false;
+  w.part = 0;
+  do {
+    if (++w.h == a.c.heads) {
+      w.h = 0;
+      ++w.b;
+      while (w.b >= blocks_of(a, w.q, RB)) {
+        w.b = 0;
+        if (++w.s >= a.r.count) return false;
+        w.q = seq_at(a.c, a.r, w.s);
+      }
+    }
+  } while (block_span(a, w.q, w.b, RB, TP).count() == 0);
+  return true;
+}
+
+template <int HDP, int NT, bool SP, bool FULL>
 __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     pack_attend_kernel(const __grid_constant__ PackAttend a, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, int spread, int parts) {
@@ -535,79 +629,42 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
   constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, MP = L::MP, TP = L::TP,
                 PITCH = L::PITCH;
   extern __shared__ __align__(1024) uint8_t sm_raw[];
-  __shared__ int red[16];
+  __shared__ int red[PACK_WARPS + 2];
   __shared__ uint64_t full[NS];
   uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
   float *fr = reinterpret_cast<float *>(sm + L::OFF_FR);
   float *wmax = reinterpret_cast<float *>(sm + L::OFF_MAX);
   float *wsum = reinterpret_cast<float *>(sm + L::OFF_SUM);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
-  const int size = a.c.size, chd = size / 32, group = a.group;
+  const int size = FULL ? HDP : a.c.size, chd = size / 32, group = a.group;
   const int wc = warp % WC, wp = warp / WC;
+  // Places in a step's codes, the swizzle resolved: piece j of this thread's
+  // key row is at kat ^ 16 j, of its two value rows at vat[.] ^ 16 j (rows a
+  // multiple of 8 on are plain offsets).
+  const int r0 = warp * 16 * MP + g8;
+  const uint32_t kat = pk_swz<PITCH>(r0, 0) + t4 * 4;
+  const uint32_t vrow = wp * (TP / WP) + 2 * t4, vj = ((wc * NB * 2) & 7) << 4;
+  const uint32_t vat[2] = {(pk_swz<PITCH>(vrow, 0) + (g8 >> 1) * 4) ^ vj, (pk_swz<PITCH>(vrow + 1, 0) + (g8 >> 1) * 4) ^ vj};
+  const uint32_t vhalf = (wc * NB / 4) * L::CODE64;  // of 512 columns, the half
+  const uint32_t zip = g8 & 1 ? 0x7632 : 0x5410;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
     mbar_init_fence();
   }
 
-  // which tiles this block takes
-  int at = 0, end = 0, s = 0, b = 0, h = 0, part = 0;
-  SeqAt q;
-  if (spread) {
-    ListAt f;
-    const int share = list_share(a, RB, TP, gridDim.x, blockIdx.x, &f, red);
-    at = blockIdx.x * share;
-    end = min(f.total, at + share);
-    pdl_release();
-    if (at >= end) return;
-    s = f.s;
-    if (s < 0) return;
-    q = seq_at(a.c, a.r, s);
-    int left = at - f.before;
-    for (;; ++b) {
-      if (b >= blocks_of(a, q, RB)) return;
-      const int n = block_span(a, q, b, RB, TP).count() * a.c.heads;
-      if (left < n) {
-        h = left / (n / a.c.heads);
-        part = left - h * (n / a.c.heads);  // the step of the unit it starts at
-        break;
-      }
-      left -= n;
-    }
-  } else {
-    const int u = blockIdx.x / parts;
-    part = blockIdx.x - u * parts;
-    h = u % a.c.heads;
-    const int total = list_total(a, RB, TP, false, 0, nullptr, red);
-    const int vb = total - 1 - u / a.c.heads;  // the rows at the end see the most: first
-    pdl_release();
-    if (vb < 0) return;
-    const ListAt f = list_at(a, RB, TP, false, vb, red);
-    s = f.s;
-    if (s < 0) return;
-    b = vb - f.before;
-    q = seq_at(a.c, a.r, s);
-  }
-
+  PackWalk w;
+  const bool any = walk_start<RB, TP>(a, spread, parts, w, red);
+  pdl_release();
+  if (!any) return;
   int step0 = 0;  // steps this block has taken: the ring's place
   bool gave_up = false;
   for (;;) {  // one unit, or a piece of it, a turn
-    const TileSpan sp = block_span(a, q, b, RB, TP);
-    const int n = sp.count();
-    int ka, kb;
-    bool whole;
-    size_t place = 0;  // of the partial sums
-    if (spread) {
-      ka = part;
-      kb = min(n, part + (end - at));
-      whole = ka == 0 && kb == n;
-      place = 2 * blockIdx.x + (ka == 0 ? 1 : 0);
-    } else {
-      ka = (int)((long)n * part / parts);
-      kb = (int)((long)n * (part + 1) / parts);
-      whole = parts == 1;
-      place = blockIdx.x;
-      if (!whole && ka == kb) return;
-    }
+    walk_unit<RB, TP>(a, spread, parts, w);
+    const SeqAt q = w.q;
+    const TileSpan sp = w.sp;
+    const int b = w.b, h = w.h, ka = w.ka, kb = w.kb;
+    const bool whole = w.whole;
+    if (!spread && !whole && ka == kb) return;
     const size_t unit = ((size_t)max(q.slot, 0) * a.c.heads + h) * a.c.positions;
     // step k's codes and scales: 64 positions a copy, those past the last
     // position any row sees left out
@@ -637,7 +694,7 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
       const bool wide = wide_rows(a.q);
       constexpr int WPL = HDP >= 256 ? HDP / 256 : 1;  // code words a lane
       for (int r = warp; r < RB; r += 4) {
-        const int rr = b * RB + r, token = rr / group, hq = h * group + rr % group;
+        const int rr = b * RB + r, token = a.by_group.of(rr), hq = h * group + rr - token * group;
         const bool live = rr < q.n * group;
         float x[WPL][8];
         float big = 0.0f;
@@ -655,13 +712,10 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
           for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[i][e]));
         }
         big = warp_max(big);
-        int ex = 0;
-        if (big > 0.0f && big <= 3.4e38f) {
-          frexpf(big, &ex);
-          ex = 14 - ex;  // big 2^ex in [2^13, 2^14)
-        }
+        const int e8 = (int)(__float_as_uint(big) >> 23);
+        const int ex = big > 0.0f && e8 < 255 ? 140 - max(e8, 1) : 0;  // big 2^ex in [2^13, 2^14)
         const float up0 = pow2i(ex / 2), up1 = pow2i(ex - ex / 2);
-        if (lane == 0) fr[r] = ldexpf(a.scale * 1.4426950408889634f, -ex);
+        if (lane == 0) fr[r] = a.scale * 1.4426950408889634f * pow2i(-(ex / 2)) * pow2i(ex / 2 - ex);
 #pragma unroll
         for (int i = 0; i < WPL; ++i) {
           const int w = lane + 32 * i, gq = w >> 2, tq = w & 3;
@@ -689,12 +743,12 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int rr = b * RB + nt * 8 + 2 * t4 + e, p = q.fill + rr / group;
+        const int rr = b * RB + nt * 8 + 2 * t4 + e, p = q.fill + a.by_group.of(rr);
         pos[nt][e] = rr < q.n * group && p < a.c.positions ? max(p, -1) : -1;
       }
-    const int p_first = q.fill + b * RB / group;  // the first row's
+    const int p_first = q.fill + a.by_group.of(b * RB);  // the first row's
     const int p_last = sp.hi - 1;
-    const bool past = q.fill + min(q.n - 1, ((b + 1) * RB - 1) / group) >= a.c.positions;
+    const bool past = q.fill + min(q.n - 1, a.by_group.of((b + 1) * RB - 1)) >= a.c.positions;
     if (tid == 0 && (past || q.slot < 0)) pack_trouble(a.c);
     __syncthreads();
 
@@ -728,29 +782,7 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[mp][nt][e] = 0.0f;
-      const int r0 = warp * 16 * MP + g8;  // and 8 on, and 16 MP on
-      uint32_t sr[MP][2][C / 2];           // the scales of its rows
-#pragma unroll
-      for (int mp = 0; mp < MP; ++mp)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint16_t *src = ksc + (r0 + mp * 16 + 8 * e) * chd;
-          if (chd == C) {
-            if constexpr (C == 2) sr[mp][e][0] = *reinterpret_cast<const uint32_t *>(src);
-            else if constexpr (C == 4) *reinterpret_cast<uint2 *>(sr[mp][e]) = *reinterpret_cast<const uint2 *>(src);
-            else {
-#pragma unroll
-              for (int i = 0; i < C / 8; ++i)
-                reinterpret_cast<uint4 *>(sr[mp][e])[i] = reinterpret_cast<const uint4 *>(src)[i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < C / 2; ++i)
-              sr[mp][e][i] = (2 * i < chd ? (uint32_t)src[2 * i] : 0u) |
-                             (2 * i + 1 < chd ? (uint32_t)src[2 * i + 1] << 16 : 0u);
-          }
-        }
-#pragma unroll
+#pragma unroll 2
       for (int gr = 0; gr < C; ++gr) {
         uint32_t aw[MP][2][4];
         float st[MP][2];
@@ -758,16 +790,15 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
         for (int mp = 0; mp < MP; ++mp) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int r = r0 + mp * 16 + 8 * e;
-            const uint8_t *box = tk + ((r >> 6) * L::HALVES + gr / 8) * L::CODE64;
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>(r & 63, gr & 7) + t4 * 4);
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(tk + (kat ^ ((gr & 7) << 4)) + (gr / 8) * L::CODE64 +
+                                                                   (mp * 16 + 8 * e) * PITCH);
             uint32_t v[4];
             dequant_i4(w, v);
             aw[mp][0][e] = v[0];
             aw[mp][0][2 + e] = v[1];
             aw[mp][1][e] = v[2];
             aw[mp][1][2 + e] = v[3];
-            st[mp][e] = __half2float(__ushort_as_half((uint16_t)(sr[mp][e][gr >> 1] >> (16 * (gr & 1)))));
+            st[mp][e] = FULL || gr < chd ? __half2float(__ushort_as_half(ksc[(r0 + mp * 16 + 8 * e) * chd + gr])) : 0.0f;
           }
         }
 #pragma unroll
@@ -781,15 +812,15 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (SP) {
               float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma16816(low, aw[mp][0], qb[L::PARTS - 1].x, qb[L::PARTS - 1].y, low);
-              mma16816(low, aw[mp][1], qb[L::PARTS - 1].z, qb[L::PARTS - 1].w, low);
-              mma16816(acc, aw[mp][0], qb[0].x, qb[0].y, acc);
-              mma16816(acc, aw[mp][1], qb[0].z, qb[0].w, acc);
+              mma_add(low, aw[mp][0], qb[L::PARTS - 1].x, qb[L::PARTS - 1].y);
+              mma_add(low, aw[mp][1], qb[L::PARTS - 1].z, qb[L::PARTS - 1].w);
+              mma_add(acc, aw[mp][0], qb[0].x, qb[0].y);
+              mma_add(acc, aw[mp][1], qb[0].z, qb[0].w);
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[e] += low[e];
             } else {
-              mma16816(acc, aw[mp][0], qb[0].x, qb[0].y, acc);
-              mma16816(acc, aw[mp][1], qb[0].z, qb[0].w, acc);
+              mma_add(acc, aw[mp][0], qb[0].x, qb[0].y);
+              mma_add(acc, aw[mp][1], qb[0].z, qb[0].w);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[mp][nt][e] = fmaf(acc[e], st[mp][e >> 1], sc[mp][nt][e]);
@@ -879,10 +910,10 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 
       // values
       constexpr int STEPS = TP / 16 / WP;
-#pragma unroll
+#pragma unroll(NT * NB <= 2 ? 2 : 1)
       for (int si = 0; si < STEPS; ++si) {
         const int st = wp * STEPS + si;
-        const int r0v = st * 16 + 2 * t4;  // this thread's positions: r0v, + 1, + 8, + 9
+        const int r0v = vrow + si * 16;  // this thread's positions: r0v, + 1, + 8, + 9
         uint2 pb[L::PARTS][NT];
 #pragma unroll
         for (int pt = 0; pt < L::PARTS; ++pt)
@@ -906,8 +937,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint16_t *src = vsc + (r0v + (i & 1) + 8 * (i >> 1)) * chd + 2 * cb;
-            if ((chd & 1) == 0) {
-              rows2[i] = 2 * cb < chd ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+            if (FULL || (chd & 1) == 0) {
+              rows2[i] = FULL || 2 * cb < chd ? *reinterpret_cast<const uint32_t *>(src) : 0u;
             } else {
               rows2[i] = (2 * cb < chd ? (uint32_t)src[0] : 0u) | (2 * cb + 1 < chd ? (uint32_t)src[1] << 16 : 0u);
             }
@@ -918,12 +949,11 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               step[i] = __byte_perm(rows2[2 * i], rows2[2 * i + 1], gi ? 0x7632 : 0x5410) & live[i];
-              const int r = r0v + 8 * i;
-              const uint8_t *box = tv + ((r >> 6) * L::HALVES + cb / 4) * L::CODE64 + (g8 >> 1) * 4;
-              const int j = (cb & 3) * 2 + gi;
-              const uint32_t w0 = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>(r & 63, j));
-              const uint32_t w1 = *reinterpret_cast<const uint32_t *>(box + pk_swz<PITCH>((r & 63) + 1, j));
-              x[i] = __byte_perm(w0, w1, g8 & 1 ? 0x7632 : 0x5410);
+              const uint8_t *box = tv + vhalf + (si * 16 + 8 * i) * PITCH;
+              const uint32_t j = (nb * 2 + gi) << 4;
+              const uint32_t w0 = *reinterpret_cast<const uint32_t *>(box + (vat[0] ^ j));
+              const uint32_t w1 = *reinterpret_cast<const uint32_t *>(box + (vat[1] ^ j));
+              x[i] = __byte_perm(w0, w1, zip);
             }
             // product u: columns 2u (rows 0-7) and 2u + 1 (rows 8-15) of the thread's four
             uint32_t av[2][4], al[2][4];
@@ -955,16 +985,16 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                  mma16816(acc, al[u], pb[0][nt].x, pb[0][nt].y, acc);
-                  mma16816(acc, av[u], pb[L::PARTS - 1][nt].x, pb[L::PARTS - 1][nt].y, acc);
-                  mma16816(acc, av[u], pb[0][nt].x, pb[0][nt].y, acc);
+                  mma_add(acc, al[u], pb[0][nt].x, pb[0][nt].y);
+                  mma_add(acc, av[u], pb[L::PARTS - 1][nt].x, pb[L::PARTS - 1][nt].y);
+                  mma_add(acc, av[u], pb[0][nt].x, pb[0][nt].y);
 #pragma unroll
                   for (int e = 0; e < 4; ++e) o[nt][nb * 4 + gi * 2 + u][e] += acc[e];
                 }
               } else {
                 const uint32_t b0 = mul2(pb[0][nt].x, step[0]), b1 = mul2(pb[0][nt].y, step[1]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) mma16816(o[nt][nb * 4 + gi * 2 + u], av[u], b0, b1, o[nt][nb * 4 + gi * 2 + u]);
+                for (int u = 0; u < 2; ++u) mma_add(o[nt][nb * 4 + gi * 2 + u], av[u], b0, b1);
               }
             }
           }
@@ -1019,7 +1049,7 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     }
     if (wp == 0) {
       const bool wide = wide_rows(a.out);
-      float *pw = a.work + place * ((size_t)RB * (size + 2));
+      float *pw = a.work + w.place * ((size_t)RB * (size + 2));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1029,8 +1059,9 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
           const float4 l4 = *reinterpret_cast<const float4 *>(wsum + r * 4);
           const float l = l4.x + l4.y + l4.z + l4.w;
           const float inv = whole ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
-          const size_t to = (size_t)(q.first + rr / group) * a.out.row_stride +
-                            (size_t)(h * group + rr % group) * a.out.head_stride;
+          const int token = a.by_group.of(rr);
+          const size_t to = (size_t)(q.first + token) * a.out.row_stride +
+                            (size_t)(h * group + rr - token * group) * a.out.head_stride;
 #pragma unroll
           for (int j = 0; j < NB * 2; ++j) {  // a group's four columns
             const int col = (wc * NB * 2 + j) * 32 + 4 * g8;
@@ -1047,26 +1078,397 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
         }
     }
 
-    // ---- the next unit
-    if (!spread) break;
-    at += kb - ka;
-    if (at >= end) break;
-    part = 0;
-    bool more = true;
-    do {
-      if (++h == a.c.heads) {
-        h = 0;
-        ++b;
-        while (more && b >= blocks_of(a, q, RB)) {
-          b = 0;
-          if (++s >= a.r.count) more = false;
-          else q = seq_at(a.c, a.r, s);
-        }
-      }
-    } while (more && block_span(a, q, b, RB, TP).count() == 0);
-    if (!more) break;
+    if (!walk_next<RB, TP>(a, spread, w)) break;
   }
   if (gave_up) pack_trouble(a.c);
+}
+
+// ---------------------------------------------------------------------------
+// attention over the codes on tcgen05, for many 16-bit query rows
+//
+// A block holds 128 query rows of one (sequence, key/value head) and the
+// whole of an SM's tensor memory: the rows' queries (f16, an operand), their
+// results (f32), and two tiles of scores whose places the weights take.  The
+// steps are tiles of 64 positions:
+//
+//   warps 4-7, 8-11  read a tile's key (value) codes a tile ahead into
+//                    registers, turn them into f16((n - 8) scale) and store
+//                    them in two operand buffers a side; rows of 64 columns
+//                    (128 bytes, swizzled), one layout for both: the key
+//                    operand's rows are its 8 KB blocks' rows, the value
+//                    operand is read across them, so nothing is transposed.
+//   warp 12          one thread issues scores (t + 1), then values (t), so
+//                    that the softmax of a tile runs beside the products of
+//                    its neighbours.
+//   warps 0-3        a thread a row: the tile's 64 scores, their maximum, the
+//                    weights back into tensor memory, the row's sum.  The
+//                    results are rescaled only when the maximum has grown by
+//                    more than 2^8 over the one in use; weights stay below
+//                    f16's range until then.
+//
+// Columns of a group of eight keep the order their nibbles come out in,
+// 0 4 1 5 2 6 3 7, in the queries and, undone at the end, in the results.
+// A query row is scaled by an exact power of two as above; keys, values and
+// weights are each rounded to f16 once (2^-11 at most).
+
+template <int HDP>
+struct PackTc {
+  static constexpr int RB = 128, TP = 64, C = HDP / 32;
+  static constexpr int BLOCKS = HDP / 64;               // 64-column blocks of an operand
+  static constexpr int SIDE = BLOCKS * 64 * 128;        // one operand buffer
+  static constexpr int T_Q = HDP, T_S = HDP + HDP / 2;  // tensor-memory columns: results, queries, scores
+  static constexpr int SMEM = 1024 + (4 * SIDE > 116 * 1024 ? 4 * SIDE : 116 * 1024);  // one block an SM
+  static constexpr int LW = C < 4 ? C : 4;              // groups across a warp's lanes
+  static constexpr int ROWS = 32 / LW;                  // positions across them
+  static constexpr int ITEMS = 64 * C / 128;            // groups a thread turns a tile
+};
+
+constexpr int TC_THREADS = 416;
+
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+// Operand descriptors, 128-byte swizzle, 8-row groups 1 KB apart: the key
+// operand along its rows (K-major), and the value operand across them
+// (MN-major: 64-column blocks 8 KB apart).
+__device__ __forceinline__ uint64_t tc_desc(uint32_t at, uint32_t lead) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+    pack_attend_tc_kernel(const __grid_constant__ PackAttend a, int spread, int parts) {
+  using L = PackTc<HDP>;
+  constexpr int RB = L::RB, TP = L::TP, C = L::C;
+  extern __shared__ __align__(1024) uint8_t tc_raw[];
+  __shared__ int red[PACK_WARPS + 2];
+  __shared__ uint64_t bars[14];
+  __shared__ uint32_t tmem_slot;
+  uint8_t *sm = tc_raw + ((1024 - (smem_u32(tc_raw) & 1023)) & 1023);
+  // [side][buffer] filled by the code warps, and free again; scores ready;
+  // weights ready; values added; queries ready
+  uint64_t *full = bars, *empty = bars + 4, *sfull = bars + 8, *pfull = bars + 10, *vdone = bars + 12, *qfull = bars + 13;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int size = a.c.size, chd = size / 32, group = a.group;
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sfull[i], 1), mbar_init(&pfull[i], 128);
+    mbar_init(vdone, 1);
+    mbar_init(qfull, 128);
+    mbar_init_fence();
+  }
+  PackWalk w;
+  const bool any = walk_start<RB, TP>(a, spread, parts, w, red);
+  pdl_release();
+  if (any) walk_unit<RB, TP>(a, spread, parts, w);
+  if (!any || (!spread && !w.whole && w.ka == w.kb)) return;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    tc_before();
+  }
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+  int step0 = 0, unit = 0;  // steps and units before this one
+  bool failed = false;
+  auto wait = [&](uint64_t *bar, int phase) {
+    if (!mbar_wait(bar, (uint32_t)(phase & 1), failed ? PACK_TRIES / 64 : PACK_TRIES)) failed = true;
+  };
+
+  for (;;) {
+    const int steps = w.kb - w.ka;
+    if (warp >= 12) {
+      // ---- the products
+      if (lane == 0 && steps > 0) {
+        constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(TP >> 3) << 17) | ((uint32_t)(RB >> 4) << 24);
+        constexpr uint32_t id_v =
+            (1u << 4) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(RB >> 4) << 24);
+        auto scores = [&](int t) {
+          const int T = step0 + t, buf = T & 1;
+          wait(&full[buf], T >> 1);
+          tc_after();
+          const uint32_t kb = smem_u32(sm + buf * L::SIDE);
+#pragma unroll
+          for (int i = 0; i < HDP / 16; ++i)
+            tc_mma_ts(tmem + L::T_S + buf * 64, tmem + L::T_Q + i * 8, tc_desc(kb + (i / 4) * 8192 + (i & 3) * 32, 16),
+                      id_s, i > 0);
+          tc_commit(&sfull[buf]);
+          tc_commit(&empty[buf]);
+        };
+        wait(qfull, unit);
+        tc_after();
+        scores(0);
+        for (int t = 0; t < steps; ++t) {
+          if (t + 1 < steps) scores(t + 1);
+          const int T = step0 + t, buf = T & 1;
+          wait(&full[2 + buf], T >> 1);
+          wait(&pfull[buf], T >> 1);
+          tc_after();
+          const uint32_t vb = smem_u32(sm + (2 + buf) * L::SIDE);
+#pragma unroll
+          for (int i = 0; i < TP / 16; ++i)
+            tc_mma_ts(tmem, tmem + L::T_S + buf * 64 + i * 8, tc_desc(vb + i * 2048, 8192), id_v, t > 0 || i > 0);
+          tc_commit(&empty[2 + buf]);
+          tc_commit(vdone);
+        }
+      }
+      __syncwarp();
+    } else if (warp >= 4) {
+      // ---- codes to operands
+      const int side = warp >= 8 ? 1 : 0, w4 = warp & 3;
+      const int row_l = lane % L::ROWS, gr_l = lane / L::ROWS;
+      const size_t base = ((size_t)max(w.q.slot, 0) * a.c.heads + w.h) * a.c.positions;
+      const uint8_t *codes = (side ? a.c.vc : a.c.kc) + base * (size / 2);
+      const uint16_t *scales = (side ? a.c.vs : a.c.ks) + base * chd;
+      uint4 code[L::ITEMS];
+      uint16_t scale[L::ITEMS];
+      // item i: a position row and a group; eight neighbouring lanes hold
+      // eight neighbouring rows, so that their stores spread over the banks
+      auto row_of = [&](int i) { return (w4 + 4 * (i / (C / L::LW))) * L::ROWS + row_l; };
+      auto group_of = [&](int i) { return gr_l + L::LW * (i % (C / L::LW)); };
+      auto fetch = [&](int t) {
+        if (t >= steps) return;
+        const int p0 = w.sp.tile(w.ka + t) * TP;
+#pragma unroll
+        for (int i = 0; i < L::ITEMS; ++i) {
+          const int p = p0 + row_of(i), gr = group_of(i);
+          code[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+          scale[i] = 0;
+          // a position no row sees counts as 0 whatever lies there
+          if (gr < chd && p < w.sp.hi && (p >= w.sp.lo || p < a.sinks)) {
+            code[i] = __ldg(reinterpret_cast<const uint4 *>(codes + (size_t)p * (size / 2)) + gr);
+            scale[i] = __ldg(scales + (size_t)p * chd + gr);
+          }
+        }
+      };
+      fetch(0);
+      for (int t = 0; t < steps; ++t) {
+        const int T = step0 + t, buf = T & 1;
+        uint4 now[L::ITEMS];
+        uint32_t by[L::ITEMS];
+#pragma unroll
+        for (int i = 0; i < L::ITEMS; ++i) now[i] = code[i], by[i] = scale[i] | ((uint32_t)scale[i] << 16);
+        fetch(t + 1);
+        if (T >= 2) wait(&empty[side * 2 + buf], (T >> 1) - 1);
+        uint8_t *dst = sm + (side * 2 + buf) * L::SIDE;
+#pragma unroll
+        for (int i = 0; i < L::ITEMS; ++i) {
+          const int r = row_of(i), gr = group_of(i);
+          uint8_t *to = dst + (gr >> 1) * 8192 + r * 128;
+          const uint32_t words[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t v[4];
+            dequant_i4(words[k], v);
+            *reinterpret_cast<uint4 *>(to + ((((gr & 1) * 4 + k) ^ (r & 7)) << 4)) =
+                make_uint4(mul2(v[0], by[i]), mul2(v[1], by[i]), mul2(v[2], by[i]), mul2(v[3], by[i]));
+          }
+        }
+        fence_async_smem();  // written here, read by the tensor core (async proxy)
+        mbar_arrive(&full[side * 2 + buf]);
+      }
+    } else {
+      // ---- the softmax, a thread a row
+      const int rr = w.b * RB + tid, token = a.by_group.of(rr), hq = w.h * group + rr - token * group;
+      const bool live = rr < w.q.n * group;
+      const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+      const int p_row = w.q.fill + token;
+      const int pos = live && p_row < a.c.positions ? max(p_row, -1) : -1;
+      const int t_last = min(w.q.n - 1, a.by_group.of((w.b + 1) * RB - 1));
+      const bool past = w.q.fill + t_last >= a.c.positions;
+      const int p_first = w.q.fill + a.by_group.of(w.b * RB), p_last = w.sp.hi - 1;
+      if (tid == 0 && (past || w.q.slot < 0)) pack_trouble(a.c);
+      float f = 0.0f;
+      if (steps > 0) {
+        const bool wide = wide_rows(a.q);
+        const size_t from = (size_t)(w.q.first + token) * a.q.row_stride + (size_t)hq * a.q.head_stride;
+        float big = 0.0f;
+        if (live)
+          for (int c = 0; c < size; c += 8) {
+            float x[8];
+            load8(a.q.data, a.q.type, from + c, wide, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+          }
+        const int e8 = (int)(__float_as_uint(big) >> 23);
+        const int ex = big > 0.0f && e8 < 255 ? 140 - max(e8, 1) : 0;  // big 2^ex in [2^13, 2^14)
+        // the scale's sign goes with the queries, so that the largest score is the largest weight's
+        const float up0 = pow2i(ex / 2), up1 = (a.scale < 0.0f ? -1.0f : 1.0f) * pow2i(ex - ex / 2);
+        f = fabsf(a.scale) * 1.4426950408889634f * pow2i(-(ex / 2)) * pow2i(ex / 2 - ex);
+        for (int c0 = 0; c0 < HDP; c0 += 64) {
+          uint32_t r[32];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float x[8] = {};
+            if (live && c0 + 8 * k < size) load8(a.q.data, a.q.type, from + c0 + 8 * k, wide, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[4 * k + e] = half2_bits(x[e] * up0 * up1, x[e + 4] * up0 * up1);
+          }
+          tc_st32(lanes + L::T_Q + c0 / 2, r);
+        }
+        tc_st_wait();
+        tc_before();
+        mbar_arrive(qfull);
+      }
+      float m = -INFINITY, l = 0.0f;  // the maximum in use (of scores as the products leave them)
+      for (int t = 0; t < steps; ++t) {
+        const int T = step0 + t, buf = T & 1;
+        wait(&sfull[buf], T >> 1);
+        tc_after();
+        uint32_t lo[32], hi[32];
+        tc_ld32(lanes + L::T_S + buf * 64, lo);
+        tc_ld32(lanes + L::T_S + buf * 64 + 32, hi);
+        tc_ld_wait();
+        const int tile0 = w.sp.tile(w.ka + t) * TP;
+        const bool all = !past && tile0 + TP - 1 <= p_first &&
+                         (a.window <= 0 || tile0 > p_last - a.window || tile0 + TP <= a.sinks);
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int j = tile0 + i;
+            if (!(j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks))) lo[i] = 0xff800000u;
+            if (!(j + 32 <= pos && (a.window <= 0 || j + 32 > pos - a.window || j + 32 < a.sinks))) hi[i] = 0xff800000u;
+          }
+        }
+        float mx[4] = {m, m, m, m};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          mx[0] = fmaxf(mx[0], __uint_as_float(lo[i]));
+          mx[1] = fmaxf(mx[1], __uint_as_float(lo[i + 1]));
+          mx[2] = fmaxf(mx[2], __uint_as_float(hi[i]));
+          mx[3] = fmaxf(mx[3], __uint_as_float(hi[i + 1]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool grown = top > m && (m == -INFINITY || (top - m) * f > 8.0f);
+        if (__any_sync(0xffffffffu, grown)) {
+          const float back = grown ? (m == -INFINITY ? 0.0f : exp2_fast((m - top) * f)) : 1.0f;
+          if (grown) m = top;
+          l *= back;
+          if (t > 0) {
+            wait(vdone, T - 1);
+            tc_after();
+#pragma unroll 1
+            for (int c = 0; c < HDP; c += 32) {
+              uint32_t r[32];
+              tc_ld32(lanes + c, r);
+              tc_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * back);
+              tc_st32(lanes + c, r);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t p[32];
+        auto weight = [&](uint32_t x) {
+          const float y = exp2_fast((__uint_as_float(x) - base) * f);  // 0 at the largest, however large
+          return all || x != 0xff800000u ? y : 0.0f;
+        };
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float x = weight(lo[i]), y = weight(lo[i + 1]);
+          p[i / 2] = half2_bits(x, y);
+          sum[0] += x;
+          sum[1] += y;
+          const float z = weight(hi[i]), v = weight(hi[i + 1]);
+          p[16 + i / 2] = half2_bits(z, v);
+          sum[2] += z;
+          sum[3] += v;
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_st32(lanes + L::T_S + buf * 64, p);
+        tc_st_wait();
+        tc_before();
+        mbar_arrive(&pfull[buf]);
+      }
+      // ---- the rows out
+      if (steps > 0) {
+        wait(vdone, step0 + steps - 1);
+        tc_after();
+      }
+      const bool wide = wide_rows(a.out);
+      const float inv = w.whole ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
+      float *pw = a.work + w.place * ((size_t)RB * (size + 2));
+      const size_t to = (size_t)(w.q.first + token) * a.out.row_stride + (size_t)hq * a.out.head_stride;
+#pragma unroll 1
+      for (int c = 0; c < size; c += 32) {
+        uint32_t r[32];
+        if (steps > 0) {
+          tc_ld32(lanes + c, r);
+          tc_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x[8] = {__uint_as_float(r[8 * k]) * inv,     __uint_as_float(r[8 * k + 2]) * inv,
+                              __uint_as_float(r[8 * k + 4]) * inv, __uint_as_float(r[8 * k + 6]) * inv,
+                              __uint_as_float(r[8 * k + 1]) * inv, __uint_as_float(r[8 * k + 3]) * inv,
+                              __uint_as_float(r[8 * k + 5]) * inv, __uint_as_float(r[8 * k + 7]) * inv};
+          if (w.whole) store8(a.out.data, a.out.type, to + c + 8 * k, wide, x);
+          else store8(pw, 1, (size_t)tid * size + c + 8 * k, true, x);
+        }
+      }
+      if (!w.whole && live) {
+        pw[(size_t)RB * size + tid] = m == -INFINITY ? -INFINITY : m * f;
+        pw[(size_t)RB * size + RB + tid] = l;
+      }
+      tc_before();
+    }
+    step0 += steps;
+    ++unit;
+    if (!walk_next<RB, TP>(a, spread, w)) break;
+    walk_unit<RB, TP>(a, spread, parts, w);
+  }
+  if (failed) pack_trouble(a.c);
+  __syncthreads();
+  if (warp == 12) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1082,7 +1484,7 @@ struct PackMerge {
 constexpr int PM_THREADS = 128, PM_CHUNK = 256;  // pieces whose factors are kept at a time
 
 __global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(PackMerge g) {
-  __shared__ int red[16];
+  __shared__ int red[PACK_WARPS + 2];
   __shared__ float pm[PM_CHUNK], pl[PM_CHUNK];
   __shared__ float4 part4[PM_THREADS];
   const PackAttend &a = g.a;
@@ -1120,7 +1522,7 @@ __global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(PackMerge g) {
     last = g.parts - 1;
     u = blockIdx.x * g.parts;
   }
-  const int rr = b * RB + r;
+  const int rr = b * RB + r, token = a.by_group.of(rr);
   const size_t piece = (size_t)RB * (size + 2);
   auto place = [&](int i) {
     return g.spread ? 2 * (size_t)i + (i * share <= u ? 1 : 0)  // the piece with the unit's first tile
@@ -1168,7 +1570,7 @@ __global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(PackMerge g) {
   }
   part4[tid] = x;
   __syncthreads();
-  if (n == 0 && tid == 0 && (q.slot < 0 || q.fill + rr / a.group >= a.c.positions)) pack_trouble(a.c);
+  if (n == 0 && tid == 0 && (q.slot < 0 || q.fill + token >= a.c.positions)) pack_trouble(a.c);
   if (team != 0) return;
   for (int i = 1; i < teams; ++i) {
     const float4 y = part4[i * lanes + tid];
@@ -1177,8 +1579,8 @@ __global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(PackMerge g) {
   const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
   const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
   store4(a.out.data, a.out.type,
-         (size_t)(q.first + rr / a.group) * a.out.row_stride +
-             (size_t)(h * a.group + rr % a.group) * a.out.head_stride + col,
+         (size_t)(q.first + token) * a.out.row_stride +
+             (size_t)(h * a.group + rr - token * a.group) * a.out.head_stride + col,
          wide_rows(a.out), y);
 }
 
@@ -1204,7 +1606,7 @@ cudaError_t pack_launch(void (*kern)(P...), dim3 grid, int threads, size_t smem,
 // its shared memory allowed and how many blocks an SM holds.
 constexpr int PACK_DEVICES = 64;
 
-template <int HDP, int NT, bool SP>
+template <int HDP, int NT, bool SP, bool FULL>
 cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
   using L = PackTile<HDP, NT, SP>;
   plan->tile = L::TP;
@@ -1214,7 +1616,7 @@ cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < PACK_DEVICES && (*per_sm = known[dev].load()) > 0) return cudaSuccess;
-  auto kern = pack_attend_kernel<HDP, NT, SP>;
+  auto kern = pack_attend_kernel<HDP, NT, SP, FULL>;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kern, 128, L::SMEM);
   if (e == cudaSuccess && *per_sm < 1) e = cudaErrorInvalidConfiguration;
@@ -1222,46 +1624,74 @@ cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
   return e;
 }
 
-template <int HDP, int NT, bool SP>
+template <int HDP, int NT, bool SP, bool FULL>
 cudaError_t pack_form_launch(const PackAttend &a, const PackPlan &p, const CUtensorMap &tmk, const CUtensorMap &tmv,
                              cudaStream_t st) {
-  return pack_launch(pack_attend_kernel<HDP, NT, SP>, dim3(p.grid), 128, PackTile<HDP, NT, SP>::SMEM, st, false, a,
+  return pack_launch(pack_attend_kernel<HDP, NT, SP, FULL>, dim3(p.grid), 128, PackTile<HDP, NT, SP>::SMEM, st, false, a,
                      tmk, tmv, p.spread, p.parts);
 }
 
 // Calls F for the form a plan names.
-#define PACK_FORMS(F, p, ...)                     \
-  switch ((p).wide * 16 + (p).rows8 * 2 + (p).split2) { \
-    case 1024 + 2 + 0: return F<64, 1, false>(__VA_ARGS__); \
-    case 1024 + 4 + 0: return F<64, 2, false>(__VA_ARGS__); \
-    case 1024 + 8 + 0: return F<64, 4, false>(__VA_ARGS__); \
-    case 1024 + 16 + 0: return F<64, 8, false>(__VA_ARGS__); \
-    case 1024 + 2 + 1: return F<64, 1, true>(__VA_ARGS__); \
-    case 1024 + 4 + 1: return F<64, 2, true>(__VA_ARGS__); \
-    case 1024 + 8 + 1: return F<64, 4, true>(__VA_ARGS__); \
-    case 2048 + 2 + 0: return F<128, 1, false>(__VA_ARGS__); \
-    case 2048 + 4 + 0: return F<128, 2, false>(__VA_ARGS__); \
-    case 2048 + 8 + 0: return F<128, 4, false>(__VA_ARGS__); \
-    case 2048 + 16 + 0: return F<128, 8, false>(__VA_ARGS__); \
-    case 2048 + 2 + 1: return F<128, 1, true>(__VA_ARGS__); \
-    case 2048 + 4 + 1: return F<128, 2, true>(__VA_ARGS__); \
-    case 2048 + 8 + 1: return F<128, 4, true>(__VA_ARGS__); \
-    case 4096 + 2 + 0: return F<256, 1, false>(__VA_ARGS__); \
-    case 4096 + 4 + 0: return F<256, 2, false>(__VA_ARGS__); \
-    case 4096 + 8 + 0: return F<256, 4, false>(__VA_ARGS__); \
-    case 4096 + 16 + 0: return F<256, 8, false>(__VA_ARGS__); \
-    case 4096 + 2 + 1: return F<256, 1, true>(__VA_ARGS__); \
-    case 4096 + 4 + 1: return F<256, 2, true>(__VA_ARGS__); \
-    case 4096 + 8 + 1: return F<256, 4, true>(__VA_ARGS__); \
-    case 8192 + 2 + 0: return F<512, 1, false>(__VA_ARGS__); \
-    case 8192 + 4 + 0: return F<512, 2, false>(__VA_ARGS__); \
-    case 8192 + 8 + 0: return F<512, 4, false>(__VA_ARGS__); \
-    case 8192 + 2 + 1: return F<512, 1, true>(__VA_ARGS__); \
-    case 8192 + 4 + 1: return F<512, 2, true>(__VA_ARGS__); \
-    default: return cudaErrorInvalidValue;        \
+#define PACK_FORMS(F, p, ...) \
+  switch ((p).wide * 32 + (p).rows8 * 4 + (p).split2 * 2 + (p).full) { \
+    case 2053: return F<64, 1, false, true>(__VA_ARGS__); \
+    case 2057: return F<64, 2, false, true>(__VA_ARGS__); \
+    case 2055: return F<64, 1, true, true>(__VA_ARGS__); \
+    case 2059: return F<64, 2, true, true>(__VA_ARGS__); \
+    case 2067: return F<64, 4, true, true>(__VA_ARGS__); \
+    case 4101: return F<128, 1, false, true>(__VA_ARGS__); \
+    case 4105: return F<128, 2, false, true>(__VA_ARGS__); \
+    case 4103: return F<128, 1, true, true>(__VA_ARGS__); \
+    case 4107: return F<128, 2, true, true>(__VA_ARGS__); \
+    case 4115: return F<128, 4, true, true>(__VA_ARGS__); \
+    case 8197: return F<256, 1, false, true>(__VA_ARGS__); \
+    case 8201: return F<256, 2, false, true>(__VA_ARGS__); \
+    case 8199: return F<256, 1, true, true>(__VA_ARGS__); \
+    case 8203: return F<256, 2, true, true>(__VA_ARGS__); \
+    case 8211: return F<256, 4, true, true>(__VA_ARGS__); \
+    case 16389: return F<512, 1, false, true>(__VA_ARGS__); \
+    case 16393: return F<512, 2, false, true>(__VA_ARGS__); \
+    case 16401: return F<512, 4, false, true>(__VA_ARGS__); \
+    case 16391: return F<512, 1, true, true>(__VA_ARGS__); \
+    case 16395: return F<512, 2, true, true>(__VA_ARGS__); \
+    case 2052: return F<64, 1, false, false>(__VA_ARGS__); \
+    case 2056: return F<64, 2, false, false>(__VA_ARGS__); \
+    case 2054: return F<64, 1, true, false>(__VA_ARGS__); \
+    case 2066: return F<64, 4, true, false>(__VA_ARGS__); \
+    case 4100: return F<128, 1, false, false>(__VA_ARGS__); \
+    case 4104: return F<128, 2, false, false>(__VA_ARGS__); \
+    case 4102: return F<128, 1, true, false>(__VA_ARGS__); \
+    case 4114: return F<128, 4, true, false>(__VA_ARGS__); \
+    case 8196: return F<256, 1, false, false>(__VA_ARGS__); \
+    case 8200: return F<256, 2, false, false>(__VA_ARGS__); \
+    case 8198: return F<256, 1, true, false>(__VA_ARGS__); \
+    case 8210: return F<256, 4, true, false>(__VA_ARGS__); \
+    case 16388: return F<512, 1, false, false>(__VA_ARGS__); \
+    case 16400: return F<512, 4, false, false>(__VA_ARGS__); \
+    case 16390: return F<512, 1, true, false>(__VA_ARGS__); \
+    case 16394: return F<512, 2, true, false>(__VA_ARGS__); \
+    default: return cudaErrorInvalidValue; \
   }
 
-static cudaError_t pack_form(PackPlan *p, int *per_sm) { PACK_FORMS(pack_form_ready, *p, p, per_sm) }
+template <int HDP>
+cudaError_t pack_tc_ready(PackPlan *plan) {
+  static std::atomic<int> known[PACK_DEVICES];
+  plan->tile = PackTc<HDP>::TP;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < PACK_DEVICES && known[dev].load())) return e;
+  e = cudaFuncSetAttribute(pack_attend_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackTc<HDP>::SMEM);
+  if (e == cudaSuccess && dev < PACK_DEVICES) known[dev].store(1);
+  return e;
+}
+
+static cudaError_t pack_form(PackPlan *p, int *per_sm) {
+  if (p->tc) {
+    *per_sm = 1;
+    return p->wide == 64 ? pack_tc_ready<64>(p) : p->wide == 128 ? pack_tc_ready<128>(p) : pack_tc_ready<256>(p);
+  }
+  PACK_FORMS(pack_form_ready, *p, p, per_sm)
+}
 static cudaError_t pack_run(const PackPlan &p, const PackAttend &a, const CUtensorMap &tmk, const CUtensorMap &tmv,
                             cudaStream_t st) {
   PACK_FORMS(pack_form_launch, p, a, p, tmk, tmv, st)
@@ -1308,10 +1738,14 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   p->wide = size <= 64 ? 64 : size <= 128 ? 128 : size <= 256 ? 256 : 512;
   p->split2 = type == 1 ? 1 : 0;
   const long need = (long)rows_most * group;
-  int most8 = p->split2 ? 4 : 8;  // what registers hold
-  if (p->wide == 512) most8 /= 2;
-  p->rows8 = need <= 8 ? 1 : need <= 16 ? 2 : need <= 32 ? 4 : 8;
-  if (p->rows8 > most8) p->rows8 = most8;
+  int most8 = p->split2 ? 4 : 2;  // what registers hold, and past 16 rows the tcgen05 form takes over
+  if (p->wide == 512) most8 = p->split2 ? 2 : 4;
+  p->full = size == p->wide;
+  p->rows8 = need <= 8 ? 1 : need <= 16 && p->full ? 2 : most8;  // fewer forms where a group's tile is part empty
+  if (!p->split2 && p->wide <= 256 && need > 16) {
+    p->tc = 1;
+    p->rows8 = 16;
+  }
   const int rb = 8 * p->rows8;
   int sms = 0, per_sm = 0;
   cudaError_t e = pack_sms(&sms);
@@ -1375,12 +1809,21 @@ static cudaError_t pack_map(const PackView &c, const void *codes, int pitch, CUt
 
 cudaError_t igc_launch_pack_attend(const PackAttend *a, const PackPlan *p, cudaStream_t st, int *launches) {
   *launches = 0;
-  CUtensorMap tmk, tmv;
-  cudaError_t e = pack_map(a->c, a->c.kc, p->pitch, &tmk);
-  if (e == cudaSuccess) e = pack_map(a->c, a->c.vc, p->pitch, &tmv);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
+  if (p->tc) {
+    auto run = [&](auto kern, int smem) {
+      return pack_launch(kern, dim3(p->grid), TC_THREADS, smem, st, false, *a, p->spread, p->parts);
+    };
+    e = p->wide == 64    ? run(pack_attend_tc_kernel<64>, PackTc<64>::SMEM)
+        : p->wide == 128 ? run(pack_attend_tc_kernel<128>, PackTc<128>::SMEM)
+                         : run(pack_attend_tc_kernel<256>, PackTc<256>::SMEM);
+  } else {
+    CUtensorMap tmk, tmv;
+    e = pack_map(a->c, a->c.kc, p->pitch, &tmk);
+    if (e == cudaSuccess) e = pack_map(a->c, a->c.vc, p->pitch, &tmv);
+    if (e == cudaSuccess) e = pack_run(*p, *a, tmk, tmv, st);
+  }
   *launches = 1;
-  e = pack_run(*p, *a, tmk, tmv, st);
   if (e != cudaSuccess || (!p->spread && p->parts == 1)) return e;
   *launches = 2;
   const PackMerge g = {*a, 8 * p->rows8, p->tile, p->spread, p->parts, p->grid, p->blocks};

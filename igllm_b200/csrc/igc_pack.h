@@ -34,11 +34,27 @@ struct PackData {
   long row_stride, head_stride;
 };
 
+// Quotients by a number known at the launch: n / d for 0 <= n < 2^31 as
+// (hi32(n mul) + n) >> shift, mul = floor(2^32 (2^shift - d) / d) + 1, 2^shift
+// the power of two from d on (Granlund and Montgomery, 1994).
+struct Quotient {
+  uint32_t mul, shift;
+#ifdef __CUDACC__
+  __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+#endif
+  static Quotient by(int d) {
+    uint32_t s = 0;
+    while ((1ull << s) < (uint64_t)d) ++s;
+    return Quotient{(uint32_t)(((1ull << 32) * ((1ull << s) - (uint64_t)d)) / (uint64_t)d + 1), s};
+  }
+};
+
 struct PackAttend {
   PackView c;
   PackRows r;
   PackData q, out;
   int group;          // query heads a key/value head
+  Quotient by_group;
   int window, sinks;  // window 0: every position up to the row's own
   float scale;
   float *work;        // split units' partial sums (PackPlan::work_floats)
@@ -46,9 +62,11 @@ struct PackAttend {
 
 // How a call's attention runs, from its host-known sizes alone.
 struct PackPlan {
-  int rows8;     // eights of query rows a block holds (1, 2, 4 or 8)
+  int rows8;     // eights of query rows a block holds (1, 2 or 4, with tc 16)
+  int tc;        // the tcgen05 form
   int wide;      // head width the kernel is built for: 64, 128, 256 or 512
   int split2;    // f32 rows: hi and lo halves of both operands
+  int full;      // the head fills that width
   int tile;      // positions a step
   int pitch;     // code bytes of a row of a TMA box
   int blocks;    // blocks a sequence can need, at most

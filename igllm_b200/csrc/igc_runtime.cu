@@ -3409,7 +3409,7 @@ extern "C" int igc_pack_attend(const igc_pack *p, const igc_pack_rows *rows, int
   if (int c = pack_plan_of(p, r, heads, q->real_type, window, sinks, &plan)) return c;
   if (plan.work_floats * sizeof(float) > work_bytes || (plan.work_floats && !work)) return IGC_FAIL_MEMORY;
   const PackAttend a = {pack_view(p), r,     pack_data_of(q), pack_data_of(out), heads / p->head_count,
-                        window,       sinks, scale,           (float *)work};
+                        Quotient::by(heads / p->head_count), window,       sinks, scale,           (float *)work};
   int launches = 0;
   const cudaError_t e = igc_launch_pack_attend(&a, &plan, (cudaStream_t)stream, &launches);
   g_launches += launches;

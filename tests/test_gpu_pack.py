@@ -10,6 +10,10 @@ Tolerances, set from the arithmetic:
   groups at most C + 8 roundings of partials no larger than
   b = scale * sum |q| * 23 * step, 2^-23 each, so a score is off by at most
   d = b (C + 8) 2^-23 and a weight by a factor e^(+-2d) after the division.
+* Where a sequence has more than 16 query rows a key/value head, of 16 bits and
+  at most 256 wide, keys are operands rounded to f16: a product is off by at
+  most 2^-11 of it, so a score by 2^-11 scale sum |q||k| more, and a weight by
+  twice that as a factor.
 * 16-bit rows: weights and values are each rounded to f16 (2^-11 of each), the
   result to its type (eps / 2).  f32 rows: hi/lo splits leave out 2^-21.
 * In the 2-norm these roundings are independent and uniform: h / sqrt(3) each.
@@ -105,6 +109,8 @@ class Setup:
                     qs = q[first + i, h * group:(h + 1) * group]
                     w = torch.softmax(qs @ k.T * scale, -1)
                     d = scale * (qs.abs() @ step.T).amax(-1) * 23 * (self.size // 32 + 8) * 2.0 ** -23
+                    if max(self.rows) * group > 16 and self.size <= 256 and self.kind != torch.float32:
+                        d += scale * (qs.abs() @ k.abs().T).amax(-1) * 2.0 ** -11 / 2
                     mass = w @ v.abs()
                     out[first + i, h * group:(h + 1) * group] = w @ v
                     each = 2.0 ** -10 + 2.0 ** -20 if self.kind != torch.float32 else 2.0 ** -19
