@@ -1,6 +1,7 @@
 // igc_pack.h - host-side launchers of igc_pack.cu: the 4-bit key/value cache.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -68,12 +69,10 @@ struct PackPlan {
   int split2;    // f32 rows: hi and lo halves of both operands
   int full;      // the head fills that width
   int tile;      // positions a step
+  int over;      // steps a unit costs beside its own
   int pitch;     // code bytes of a row of a TMA box
-  int blocks;    // blocks a sequence can need, at most
-  int spread;    // 1: one list of tiles over all units, an equal share a block; 0: `parts` blocks a unit
-  int parts;
+  int tall;      // some sequence has many blocks of rows
   int grid;
-  int units;     // (block, key/value head) units the grid and the merge cover
   size_t work_floats;
 };
 
@@ -87,6 +86,10 @@ cudaError_t igc_launch_pack_read(const igc::PackView *c, const igc::PackRows *r,
 // `type` the query rows' type, `rows_most` the most rows of any sequence.
 cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int kv_heads, int group, int size,
                           int type, int window, int sinks, igc::PackPlan *plan);
+// igc_pack_tc.cu's part of the two calls around it.
+cudaError_t igc_pack_tc_ready(igc::PackPlan *plan);
+cudaError_t igc_launch_pack_tc(const igc::PackAttend *a, const igc::PackPlan *plan, const CUtensorMap *keys,
+                               const CUtensorMap *values, cudaStream_t st);
 cudaError_t igc_launch_pack_attend(const igc::PackAttend *a, const igc::PackPlan *plan, cudaStream_t st,
                                    int *launches);
 }
