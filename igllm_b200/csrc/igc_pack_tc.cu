@@ -35,7 +35,7 @@ namespace igc {
 template <int HDP>
 struct PackTc {
   static constexpr int RB = 128, TP = 64, C = HDP / 32;
-  static constexpr int OVER = 10;                       // steps a unit costs beside its own
+  static constexpr int OVER = 8;                        // steps a unit costs beside its own
   static constexpr int BLOCKS = HDP / 64;               // 64-column blocks of an operand
   static constexpr int SIDE = BLOCKS * 64 * 128;        // one key or value operand buffer
   static constexpr int T_S = HDP;                       // tensor-memory columns: results, then four tiles of scores
@@ -104,6 +104,11 @@ __device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&r)[16]) {
       : "r"(at));
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+// 16 bytes (or, of none, zeros) into shared memory, not waited for.
+__device__ __forceinline__ void pk_copy16(void *dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
 
 // Pairs of floats at once.
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
@@ -389,19 +394,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           float big = 0.0f;
           if (!idle) {
             const long at = live ? (long)(u.q_first + token) * a.q.row_stride + (long)hq * a.q.head_stride : -1;
-#pragma unroll 8
-            for (int i = 0; i < PIECES; ++i) {
-              const long from = row_at(at, i);
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (from >= 0 && my_col < size) {
-                const uint16_t *p = static_cast<const uint16_t *>(a.q.data) + from + my_col;
-                if (wide)
-                  v = *reinterpret_cast<const uint4 *>(p);
-                else
-                  v = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16,
-                                 p[6] | (uint32_t)p[7] << 16);
+            const uint16_t *src = static_cast<const uint16_t *>(a.q.data);
+            if (wide) {
+#pragma unroll
+              for (int i = 0; i < PIECES; ++i) {
+                const long from = row_at(at, i);
+                const bool have = from >= 0 && my_col < size;
+                pk_copy16(piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece), src + (have ? from + my_col : 0),
+                          have ? 16 : 0);
               }
-              *piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece) = v;
+              asm volatile("cp.async.wait_all;\n" ::: "memory");
+            } else {
+#pragma unroll 1
+              for (int i = 0; i < PIECES; ++i) {
+                const long from = row_at(at, i);
+                const uint16_t *p = src + from + my_col;
+                *piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece) =
+                    from >= 0 && my_col < size ? make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16,
+                                                            p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16)
+                                               : make_uint4(0, 0, 0, 0);
+              }
             }
             __syncwarp();
             if (bf) {
@@ -557,48 +569,70 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (!idle) {
           const bool wide = wide_rows(a.out), whole = u.whole;
           const float inv = whole ? (l == 0.0f ? 0.0f : __fdividef(1.0f, l)) : 1.0f;
-          float *pw = u.piece;
+          const long at = !live  ? -1
+                          : whole ? (long)(u.q_first + token) * a.out.row_stride + (long)hq * a.out.head_stride
+                                  : (long)r * size;
+          // 16 bits: the half's columns at once; partial sums, in 32: half of
+          // them at a time (of a 64-wide head straight from the registers)
+          constexpr int PART = HDP > 64 ? HDP / 4 : 32;
+          for (int c0 = half * (HDP / 2); c0 < min(size, (half + 1) * (HDP / 2)); c0 += whole ? HDP / 2 : PART) {
 #pragma unroll 1
-          for (int c = half * (HDP / 2); c < min(size, (half + 1) * (HDP / 2)); c += 32) {
-            uint32_t o[32];
-            if (steps > 0) {
-              tc_ld32(lanes + c, o);
-              tc_ld_wait();
+            for (int k = 0; k < (whole ? HDP / 2 : PART) / 32; ++k) {
+              uint32_t o[32];
+              if (steps > 0) {
+                tc_ld32(lanes + c0 + 32 * k, o);
+                tc_ld_wait();
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0;
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y[8] = {__uint_as_float(o[8 * e]) * inv,     __uint_as_float(o[8 * e + 2]) * inv,
+                                    __uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 6]) * inv,
+                                    __uint_as_float(o[8 * e + 1]) * inv, __uint_as_float(o[8 * e + 3]) * inv,
+                                    __uint_as_float(o[8 * e + 5]) * inv, __uint_as_float(o[8 * e + 7]) * inv};
+                if (whole) {
+                  store8(piece_of(r, 4 * k + e), a.out.type, 0, true, y);
+                } else if (HDP == 64) {
+                  if (live) store8(u.piece, 1, at + c0 + 8 * e, true, y);
+                } else {
+                  *reinterpret_cast<float4 *>(piece_of(r, 8 * k + 2 * e)) = make_float4(y[0], y[1], y[2], y[3]);
+                  *reinterpret_cast<float4 *>(piece_of(r, 8 * k + 2 * e + 1)) = make_float4(y[4], y[5], y[6], y[7]);
+                }
+              }
+            }
+            if (!whole && HDP == 64) continue;
+            __syncwarp();
+            const int col = c0 + (whole ? 8 : 4) * my_piece;
+            const bool in = col < size;
+            if (whole && !wide) {
+#pragma unroll 1
+              for (int i = 0; i < PIECES; ++i) {
+                const long to = row_at(at, i);
+                const uint4 v = *piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece);
+                uint16_t *p = static_cast<uint16_t *>(a.out.data) + to + col;
+                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                if (to >= 0 && in) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) p[2 * e] = (uint16_t)x[e], p[2 * e + 1] = (uint16_t)(x[e] >> 16);
+                }
+              }
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float y[8] = {__uint_as_float(o[8 * k]) * inv,     __uint_as_float(o[8 * k + 2]) * inv,
-                                  __uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 6]) * inv,
-                                  __uint_as_float(o[8 * k + 1]) * inv, __uint_as_float(o[8 * k + 3]) * inv,
-                                  __uint_as_float(o[8 * k + 5]) * inv, __uint_as_float(o[8 * k + 7]) * inv};
-              if (whole) store8(piece_of(r, c / 8 - half * PIECES + k), a.out.type, 0, true, y);
-              else if (live) store8(pw, 1, (size_t)r * size + c + 8 * k, true, y);
-            }
-          }
-          if (whole) {
-            const long at = live ? (long)(u.q_first + token) * a.out.row_stride + (long)hq * a.out.head_stride : -1;
-            __syncwarp();
-#pragma unroll 4
-            for (int i = 0; i < PIECES; ++i) {
-              const long to = row_at(at, i);
-              const uint4 v = *piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece);
-              if (to < 0 || my_col >= size) continue;
-              uint16_t *p = static_cast<uint16_t *>(a.out.data) + to + my_col;
-              if (wide) {
-                *reinterpret_cast<uint4 *>(p) = v;
-              } else {
-                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[2 * e] = (uint16_t)x[e], p[2 * e + 1] = (uint16_t)(x[e] >> 16);
+              for (int i = 0; i < PIECES; ++i) {
+                const long to = row_at(at, i);
+                const uint4 v = *piece_of((r & 96) + i * AT_ONCE + lane / PIECES, my_piece);
+                uint4 *p = whole ? reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out.data) + to + col)
+                                 : reinterpret_cast<uint4 *>(u.piece + to + col);
+                if (to >= 0 && in) *p = v;
               }
             }
             __syncwarp();
-          } else if (live && !half) {
-            pw[(size_t)RB * size + r] = m == -INFINITY ? -INFINITY : m * f;
-            pw[(size_t)RB * size + RB + r] = l;
+          }
+          if (!whole && live && !half) {
+            u.piece[(size_t)RB * size + r] = m == -INFINITY ? -INFINITY : m * f;
+            u.piece[(size_t)RB * size + RB + r] = l;
           }
         }
         tc_before();
