@@ -661,6 +661,9 @@ class PackCache:
         self._p = IgcPack(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
                           value_scales.data_ptr(), slots, heads, positions, 2 * half, self.device.index,
                           self._trouble.data_ptr())
+        self._index = self.device.index
+        self._int32 = torch.int32
+        self._raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, no object made
         self._room = {}  # scratch bytes by a call's sizes
         if positions % PACK_TILE or self.size % PACK_GROUP or not PACK_GROUP <= self.size <= 512:
             raise ValueError(f"PackCache: {positions} positions (a multiple of {PACK_TILE}) of {self.size} values "
@@ -684,8 +687,7 @@ class PackCache:
     def _list(self, t, name, n):
         if t is None:
             return None
-        if t.dtype != self._torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or \
-                t.device != self.device:
+        if t.dtype is not self._int32 or t.shape != (n,) or t.device != self.device or (n > 1 and t.stride(0) != 1):
             raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not {n} int32 on "
                              f"{self.device}")
         return t.data_ptr()
@@ -705,7 +707,7 @@ class PackCache:
         return IgcPackData(t.data_ptr(), self._types[t.dtype], row, head)
 
     def _stream(self):
-        return self._torch.cuda.current_stream(self.device).cuda_stream
+        return self._raw_stream(self._index)
 
     def write(self, keys, values, fill, starts=None, slots=None, rows_most=None):
         """Rows [n, heads, size] quantised into their places."""
@@ -720,7 +722,7 @@ class PackCache:
         """(keys, values) of `rows` rows decoded, [rows, heads, size] of `dtype`
         (in arrays made here, rows of no sequence hold nothing of meaning)."""
         if out is None:
-            out = tuple(self._torch.empty((rows, self.heads, self.size), dtype=dtype, device=self.device) for _ in range(2))
+            out = fill.new_empty((2, rows, self.heads, self.size), dtype=dtype).unbind(0)
         if rows:
             _check(_lib().igc_pack_read(self._p, self._rows(rows, fill, starts, slots, rows_most),
                                         self._data(out[0], "keys", rows, self.heads),
@@ -733,7 +735,7 @@ class PackCache:
         only the last `window` of them and the first `sinks` of all."""
         n, heads = queries.shape[0], queries.shape[1]
         if out is None:
-            out = self._torch.empty(queries.shape, dtype=queries.dtype, device=queries.device)
+            out = queries.new_empty(queries.shape)
         if n == 0:
             return out
         rows = self._rows(n, fill, starts, slots, rows_most)
@@ -747,7 +749,7 @@ class PackCache:
             if len(self._room) > 4096:
                 self._room.clear()
             room = self._room[key] = need.value
-        work = self._torch.empty(room, dtype=self._torch.uint8, device=self.device) if room else None
+        work = self.key_codes.new_empty(room) if room else None
         _check(_lib().igc_pack_attend(self._p, rows, heads, q, o, window, sinks, scale,
                                       work.data_ptr() if room else None, room, self._stream()), "pack_attend")
         return out

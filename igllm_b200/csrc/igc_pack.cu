@@ -29,85 +29,170 @@
 namespace igc {
 
 // ---------------------------------------------------------------------------
-// write and read: one thread a code word (8 columns), four threads a group.
-// Both are one pass over their rows, bound by HBM.
+// write and read: a thread half a group (two code words), two of them a turn
+// with their loads issued together, a block the rows of one side and head,
+// whose places are neighbours.  Both are one pass over their rows, bound
+// by HBM where instructions allow: a code is rint(x / scale), the division
+// IEEE's, but it is only divided where x times the reciprocal comes within
+// 2e-6 of a tie (it is off by at most 8 2^-23); a group that
+// holds a NaN or needs the clamp takes the long way too.
 
-constexpr int PK_THREADS = 256, PK_ITEMS = 4;
+constexpr int PK_THREADS = 256, PK_ITEMS = 2, PK_TURNS = 2, PK_COLS = 16;
 
 struct PackIo {
   PackView c;
   PackRows r;
   PackData k, v;
+  int halves, rows;              // a head's halves of groups; rows a block takes at a time
+  Quotient by_halves, by_per;    // and rows a sequence
 };
 
-template <bool WRITE>
-__global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(PackIo a) {
-  const int words = a.c.size / 8, row_words = 2 * a.c.heads * words;
-  const long first = (long)blockIdx.x * (PK_THREADS * PK_ITEMS);
-  const int row0 = (int)(first / row_words), rem0 = (int)(first - (long)row0 * row_words);
-  const bool kwide = wide_rows(a.k), vwide = wide_rows(a.v);
-  int s = -1;
+// The last sequence that starts at or before `row`, the same for the warp.
+__device__ __forceinline__ int seq_before(const PackRows &r, int row) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int i = lane; i < r.count; i += 32) n += r.starts[i] <= row;
+  return max((int)__reduce_add_sync(0xffffffffu, n) - 1, 0);
+}
+
+__device__ __forceinline__ float max_nan(float x, float y) {  // a NaN where either is one
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// x over a scale, to a whole number: the definition, kept out of the way.
+__device__ __noinline__ float code_of(float x, float step) { return rintf(__fdiv_rn(x, step)); }
+
+// The codes of 16 values, and the scale of their group (two neighbouring
+// lanes hold it).
+__device__ __forceinline__ uint2 encode16(const float (&x)[PK_COLS], __half *scale) {
+  const uint32_t pair = 3u << (threadIdx.x & 30);
+  float big = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PK_COLS; ++i) big = max_nan(big, fabsf(x[i]));
+  big = max_nan(big, __shfl_xor_sync(pair, big, 1));
+  const bool odd = big != big;
+  if (odd) {  // without the NaNs
+    big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PK_COLS; ++i) big = fmaxf(big, fabsf(x[i]));
+    big = fmaxf(big, __shfl_xor_sync(pair, big, 1));
+  }
+  const __half h = __float2half_rn(fminf(__fdiv_rn(big, 7.0f), 8188.0f));
+  const float step = __half2float(h), by = __frcp_rn(step);
+  *scale = h;
+  uint32_t w[2] = {0, 0};
+  if (!odd && big * by < 7.4f) {
+#pragma unroll
+    for (int i = PK_COLS - 1; i >= 0; --i) {
+      const float r = x[i] * by;
+      float y = r + 12582920.0f;  // 1.5 2^23 + 8: rounded to a whole number, its low bits n + 8
+      if (fabsf(r - (y - 12582920.0f)) > 0.499998f) y = code_of(x[i], step) + 12582920.0f;
+      w[i >> 3] = w[i >> 3] * 16 + (__float_as_uint(y) & 15u);
+    }
+  } else {
+    w[0] = w[1] = 0;
+#pragma unroll 1
+    for (int i = PK_COLS - 1; i >= 0; --i) {
+      float v = x[0];  // x[i], with no array in memory
+#pragma unroll
+      for (int k = 1; k < PK_COLS; ++k) v = k == i ? x[k] : v;
+      float n = step > 0.0f && v == v ? code_of(v, step) : 0.0f;
+      n = fminf(fmaxf(n, -8.0f), 7.0f);
+      const uint32_t c = (uint32_t)((int)n + 8);
+      if (i >= 8) w[1] = w[1] * 16 + c;
+      else w[0] = w[0] * 16 + c;
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// Eight codes' values.
+__device__ __forceinline__ void decode8(uint32_t w, float step, float (&x)[8]) {
+  uint32_t v[4];
+  dequant_i4(w, v);  // codes e and e + 4 together
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v[e]));
+    x[e] = f.x * step;
+    x[e + 4] = f.y * step;
+  }
+}
+
+template <bool WRITE, int TYPE, bool WIDE>
+__global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_constant__ PackIo a) {
+  const int side = blockIdx.y & 1, head = blockIdx.y >> 1;
+  const int r = a.by_halves.of(threadIdx.x), w = threadIdx.x - r * a.halves;
+  const PackData d = side ? a.v : a.k;
+  uint2 *codes = reinterpret_cast<uint2 *>(side ? a.c.vc : a.c.kc);
+  uint16_t *scales = side ? a.c.vs : a.c.ks;
+  const size_t col = (size_t)head * d.head_stride + PK_COLS * w;
+  int row = blockIdx.x * (a.rows * PK_ITEMS * PK_TURNS) + r;
+  int s = a.r.starts ? seq_before(a.r, min(row - r, a.r.rows - 1)) : 0;
+  if (r >= a.rows) return;  // threads past a whole number of rows
   SeqAt q = {0, 0, 0, -1};
+  bool have = false;
+#pragma unroll 1
+  for (int turn = 0; turn < PK_TURNS; ++turn) {
+    // 0 nothing to do, 1 a place of the cache, 2 zeros (padding, or outside the cache), by item
+    int todo[PK_ITEMS];
+    size_t at[PK_ITEMS], half_at[PK_ITEMS];
 #pragma unroll
-  for (int it = 0; it < PK_ITEMS; ++it) {
-    const int off = rem0 + it * PK_THREADS + threadIdx.x;
-    const int row = row0 + off / row_words;
-    if (row >= a.r.rows) return;  // whole groups leave together: a row is a multiple of four words
-    int rest = off % row_words;
-    const int side = rest / (a.c.heads * words);
-    rest -= side * a.c.heads * words;
-    const int head = rest / words, w = rest - head * words;
-    if (s < 0 || row < q.first || row >= q.first + q.n) {
-      s = seq_of_row(a.r, row);
-      q = seq_at(a.c, a.r, s);
-    }
-    if (row < q.first || row >= q.first + q.n) continue;  // no sequence's row
-    const int p = q.fill + (row - q.first);
-    if (p < 0) {  // padding
-      if (!WRITE) {
-        const float zero[8] = {};
-        const PackData &d = side ? a.v : a.k;
-        store8(d.data, d.type, (size_t)row * d.row_stride + (size_t)head * d.head_stride + 8 * w, side ? vwide : kwide,
-               zero);
+    for (int it = 0; it < PK_ITEMS; ++it, row += a.rows) {
+      todo[it] = 0;
+      if (row >= a.r.rows) continue;
+      if (!a.r.starts) {
+        const int now = a.by_per.of(row);
+        if (!have || now != s) q = seq_at(a.c, a.r, s = now), have = true;
+      } else {
+        if (!have) q = seq_at(a.c, a.r, s), have = true;
+        while (row >= a.r.starts[s + 1] && s + 1 < a.r.count) q = seq_at(a.c, a.r, ++s);
       }
-      continue;
+      if (row < q.first || row >= q.first + q.n) continue;  // no sequence's row
+      const int p = q.fill + (row - q.first);
+      const bool outside = p >= a.c.positions || q.slot < 0;
+      if (p >= 0 && outside) pack_trouble(a.c);
+      todo[it] = p < 0 || outside ? 2 : 1;
+      at[it] = (size_t)row * d.row_stride + col;
+      half_at[it] = (todo[it] == 1 ? ((size_t)q.slot * a.c.heads + head) * a.c.positions + p : 0) * a.halves + w;
     }
-    const bool out = q.slot < 0 || p >= a.c.positions;
-    if (out) {
-      pack_trouble(a.c);
-      if (WRITE) continue;
-    }
-    const PackData &d = side ? a.v : a.k;
-    const size_t at = (size_t)row * d.row_stride + (size_t)head * d.head_stride + 8 * w;
-    const size_t place = ((size_t)(out ? 0 : q.slot) * a.c.heads + head) * a.c.positions + (out ? 0 : p);
-    uint32_t *code = reinterpret_cast<uint32_t *>(side ? a.c.vc : a.c.kc) + place * words + w;
-    uint16_t *scale = (side ? a.c.vs : a.c.ks) + place * (words / 4) + (w >> 2);
-    float x[8];
     if (WRITE) {
-      load8(d.data, d.type, at, side ? vwide : kwide, x);
-      float big = 0.0f;
+      float x[PK_ITEMS][PK_COLS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));  // a NaN does not take part
-      const uint32_t four = 0xfu << (threadIdx.x & 28);
-      big = fmaxf(big, __shfl_xor_sync(four, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(four, big, 2));
-      const __half h = __float2half_rn(fminf(__fdiv_rn(big, 7.0f), 8188.0f));
-      const float step = __half2float(h);
-      uint32_t word = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float n = step > 0.0f && x[i] == x[i] ? rintf(__fdiv_rn(x[i], step)) : 0.0f;
-        n = fminf(fmaxf(n, -8.0f), 7.0f);
-        word |= (uint32_t)((int)n + 8) << (4 * i);
+      for (int it = 0; it < PK_ITEMS; ++it) {
+        if (todo[it] != 1) continue;
+        load8(d.data, TYPE, at[it], WIDE, *reinterpret_cast<float(*)[8]>(&x[it][0]));
+        load8(d.data, TYPE, at[it] + 8, WIDE, *reinterpret_cast<float(*)[8]>(&x[it][8]));
       }
-      *code = word;
-      if ((w & 3) == 0) *scale = __half_as_ushort(h);
-    } else {
-      const uint32_t word = out ? 0x88888888u : *code;
-      const float step = out ? 0.0f : __half2float(__ushort_as_half(*scale));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)((int)((word >> (4 * i)) & 15u) - 8) * step;
-      store8(d.data, d.type, at, side ? vwide : kwide, x);
+      for (int it = 0; it < PK_ITEMS; ++it) {
+        if (todo[it] != 1) continue;
+        __half h;
+        codes[half_at[it]] = encode16(x[it], &h);
+        if ((w & 1) == 0) scales[half_at[it] >> 1] = __half_as_ushort(h);
+      }
+    } else {
+      uint2 c[PK_ITEMS];
+      float step[PK_ITEMS];
+#pragma unroll
+      for (int it = 0; it < PK_ITEMS; ++it) {
+        c[it] = make_uint2(0x88888888u, 0x88888888u);
+        step[it] = 0.0f;
+        if (todo[it] == 1) {
+          c[it] = codes[half_at[it]];
+          step[it] = __half2float(__ushort_as_half(scales[half_at[it] >> 1]));
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < PK_ITEMS; ++it) {
+        if (todo[it] == 0) continue;
+        float x[8];
+        decode8(c[it].x, step[it], x);
+        store8(d.data, TYPE, at[it], WIDE, x);
+        decode8(c[it].y, step[it], x);
+        store8(d.data, TYPE, at[it] + 8, WIDE, x);
+      }
     }
   }
 }
@@ -854,24 +939,41 @@ static cudaError_t pack_sms(int *sms) {
 
 using namespace igc;
 
-static cudaError_t launch_rows(bool write, const PackView *c, const PackRows *r, const PackData *k, const PackData *v,
+template <bool WRITE>
+static cudaError_t launch_rows(const PackView *c, const PackRows *r, const PackData *k, const PackData *v,
                                cudaStream_t st) {
-  const PackIo io = {*c, *r, *k, *v};
-  const long items = (long)r->rows * 2 * c->heads * (c->size / 8);
-  const long blocks = (items + PK_THREADS * PK_ITEMS - 1) / (PK_THREADS * PK_ITEMS);
-  if (blocks < 1 || blocks > 0x7fffffffL) return cudaErrorInvalidValue;
-  return write ? pack_launch(pack_rows_kernel<true>, dim3((unsigned)blocks), PK_THREADS, 0, st, false, io)
-               : pack_launch(pack_rows_kernel<false>, dim3((unsigned)blocks), PK_THREADS, 0, st, false, io);
+  if (k->type != v->type) return cudaErrorInvalidValue;
+  const int halves = c->size / PK_COLS;
+  const int rows = PK_THREADS / halves;
+  const PackIo io = {*c, *r, *k, *v, halves, rows, Quotient::by(halves), Quotient::by(r->per > 0 ? r->per : 1)};
+  const int block_rows = rows * PK_ITEMS * PK_TURNS;
+  const dim3 grid((unsigned)((r->rows + block_rows - 1) / block_rows), 2 * c->heads);
+  if (c->heads > 32767) return cudaErrorInvalidValue;
+  // 16 bytes at a time where every eight columns of both sides start on them
+  auto lies = [](const PackData &d) {
+    const long per = d.type == 1 ? 4 : 8;
+    return ((size_t)d.data & 15) == 0 && d.row_stride % per == 0 && d.head_stride % per == 0;
+  };
+  const bool wide = lies(*k) && lies(*v);
+  auto run = [&](auto kern) { return pack_launch(kern, grid, PK_THREADS, 0, st, false, io); };
+  switch (k->type * 2 + (wide ? 1 : 0)) {
+    case 2: return run(pack_rows_kernel<WRITE, 1, false>);
+    case 3: return run(pack_rows_kernel<WRITE, 1, true>);
+    case 4: return run(pack_rows_kernel<WRITE, 2, false>);
+    case 5: return run(pack_rows_kernel<WRITE, 2, true>);
+    case 6: return run(pack_rows_kernel<WRITE, 3, false>);
+    default: return run(pack_rows_kernel<WRITE, 3, true>);
+  }
 }
 
 cudaError_t igc_launch_pack_write(const PackView *c, const PackRows *r, const PackData *k, const PackData *v,
                                   cudaStream_t st) {
-  return launch_rows(true, c, r, k, v, st);
+  return launch_rows<true>(c, r, k, v, st);
 }
 
 cudaError_t igc_launch_pack_read(const PackView *c, const PackRows *r, const PackData *k, const PackData *v,
                                  cudaStream_t st) {
-  return launch_rows(false, c, r, k, v, st);
+  return launch_rows<false>(c, r, k, v, st);
 }
 
 cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int kv_heads, int group, int size,

@@ -42,19 +42,6 @@ __device__ __forceinline__ SeqAt seq_at(const PackView &c, const PackRows &r, in
   return q;
 }
 
-// The sequence that holds `row`, or -1: the last whose rows start at or
-// before it, if they reach it.
-__device__ __forceinline__ int seq_of_row(const PackRows &r, int row) {
-  if (!r.starts) return row / r.per;
-  int lo = 0, hi = r.count;  // starts[lo] <= row < starts[hi], where that holds at all
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (r.starts[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // ---------------------------------------------------------------------------
 // rows of values
 

@@ -3308,7 +3308,7 @@ bool pack_sane(const igc_pack *p) {
   if (p->slot_count < 1 || p->head_count < 1 || p->position_count < PACK_TILE || p->position_count % PACK_TILE != 0)
     return false;
   if (p->head_size < PACK_GROUP || p->head_size > 512 || p->head_size % PACK_GROUP != 0) return false;
-  if (p->device < 0 || p->head_count > (1 << 16)) return false;
+  if (p->device < 0 || p->head_count > 32767) return false;
   return (double)p->slot_count * p->head_count * p->position_count < 2147483648.0;  // positions are counted in ints
 }
 
@@ -3345,6 +3345,7 @@ PackData pack_data_of(const igc_pack_data *d) {
 int pack_move(bool write, const igc_pack *p, const igc_pack_rows *rows, const igc_pack_data *k,
               const igc_pack_data *v, void *stream) {
   if (!pack_sane(p) || !pack_rows_sane(p, rows) || !pack_data_sane(k) || !pack_data_sane(v)) return IGC_FAIL_ARGUMENT;
+  if (k->real_type != v->real_type) return IGC_FAIL_ARGUMENT;
   if (rows->row_count == 0) return IGC_OKAY;
   clear_stale("pack rows");
   DeviceScope dev(p->device);

@@ -372,8 +372,8 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * igc_pack_data is an array of rows: `real_type` 1 F32, 2 F16, 3 BF16 (the
  * reference's store_type values), strides in values, a head's values adjacent.
  *
- * igc_pack_write: keys and values (row_count x head_count x head_size) into
- * their places.  igc_pack_read: the same places decoded.
+ * igc_pack_write: keys and values (row_count x head_count x head_size, of one
+ * type) into their places.  igc_pack_read: the same places decoded.
  *
  * igc_pack_attend: for each row at position p and each of `head_count` query
  * heads (head h reads key/value head h / (head_count / pack->head_count)),

@@ -71,6 +71,13 @@ def test_bad_attention_is_refused(igc_lib):
         assert call(p, r, None, d, None) == igc_lib.FAIL_ARGUMENT
 
 
+def test_keys_and_values_have_one_type(igc_lib):
+    lib = igc_lib._lib()
+    p, r, d = _pack(igc_lib), _rows(igc_lib), _data(igc_lib)
+    for call in (lib.igc_pack_write, lib.igc_pack_read):
+        assert call(p, r, d, _data(igc_lib, real_type=2), None) == igc_lib.FAIL_ARGUMENT
+
+
 def test_no_rows_is_no_call(igc_lib):
     lib = igc_lib._lib()
     p, d = _pack(igc_lib), _data(igc_lib)
