@@ -32,10 +32,10 @@ namespace igc {
 // write and read: a thread half a group (two code words), two of them a turn
 // with their loads issued together, a block the rows of one side and head,
 // whose places are neighbours.  Both are one pass over their rows, bound
-// by HBM where instructions allow: a code is rint(x / scale), the division
-// IEEE's, but it is only divided where x times the reciprocal comes within
-// 2e-6 of a tie (it is off by at most 8 2^-23); a group that
-// holds a NaN or needs the clamp takes the long way too.
+// by HBM where instructions allow.  A code is rint(x / scale) with the quotient
+// rounded as IEEE's division does, which Markstein's correction (1990) gives
+// from the correctly rounded reciprocal: q = x y, then q + (x - q scale) y with
+// fused multiply-adds.  A group that holds a NaN or needs the clamp divides.
 
 constexpr int PK_THREADS = 256, PK_ITEMS = 2, PK_TURNS = 2, PK_COLS = 16;
 
@@ -61,9 +61,6 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // a NaN where eit
   return z;
 }
 
-// x over a scale, to a whole number: the definition, kept out of the way.
-__device__ __noinline__ float code_of(float x, float step) { return rintf(__fdiv_rn(x, step)); }
-
 // The codes of 16 values, and the scale of their group (two neighbouring
 // lanes hold it).
 __device__ __forceinline__ uint2 encode16(const float (&x)[PK_COLS], __half *scale) {
@@ -86,9 +83,8 @@ __device__ __forceinline__ uint2 encode16(const float (&x)[PK_COLS], __half *sca
   if (!odd && big * by < 7.4f) {
 #pragma unroll
     for (int i = PK_COLS - 1; i >= 0; --i) {
-      const float r = x[i] * by;
-      float y = r + 12582920.0f;  // 1.5 2^23 + 8: rounded to a whole number, its low bits n + 8
-      if (fabsf(r - (y - 12582920.0f)) > 0.499998f) y = code_of(x[i], step) + 12582920.0f;
+      const float r = x[i] * by, quotient = fmaf(fmaf(-r, step, x[i]), by, r);
+      const float y = quotient + 12582920.0f;  // 1.5 2^23 + 8: rounded to a whole number, its low bits n + 8
       w[i >> 3] = w[i >> 3] * 16 + (__float_as_uint(y) & 15u);
     }
   } else {
@@ -98,7 +94,7 @@ __device__ __forceinline__ uint2 encode16(const float (&x)[PK_COLS], __half *sca
       float v = x[0];  // x[i], with no array in memory
 #pragma unroll
       for (int k = 1; k < PK_COLS; ++k) v = k == i ? x[k] : v;
-      float n = step > 0.0f && v == v ? code_of(v, step) : 0.0f;
+      float n = step > 0.0f && v == v ? rintf(__fdiv_rn(v, step)) : 0.0f;
       n = fminf(fmaxf(n, -8.0f), 7.0f);
       const uint32_t c = (uint32_t)((int)n + 8);
       if (i >= 8) w[1] = w[1] * 16 + c;
