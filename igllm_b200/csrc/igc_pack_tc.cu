@@ -324,42 +324,51 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         const int row_l = lane % L::ROWS, gr_l = lane / L::ROWS;
         const uint8_t *ring = sm + L::OFF_CODE;
         // item i: a position row and a group; eight neighbouring lanes hold
-        // eight neighbouring rows, so that their accesses spread over the banks
-        auto row_of = [&](int i) { return (w4 + 4 * (i / (C / L::LW))) * L::ROWS + row_l; };
-        auto group_of = [&](int i) { return gr_l + L::LW * (i % (C / L::LW)); };
+        // eight neighbouring rows, so that their accesses spread over the
+        // banks.  Items are plain offsets apart: ACROSS groups to a row, then
+        // rows; the swizzles are resolved here once.
+        constexpr int ACROSS = C / L::LW, DOWN = 4 * L::ROWS;
+        const int r0 = w4 * L::ROWS + row_l;
+        const uint32_t src0 = pk_swz<L::PITCH>(r0, gr_l), sc0 = (uint32_t)(64 * L::PITCH + (r0 * chd + gr_l) * 2);
+        const uint32_t dst0 = (uint32_t)((gr_l >> 1) * 8192 + r0 * 128 + ((((gr_l & 1) * 4) ^ (r0 & 7)) << 4));
         const int hi = u.hi, lo = u.lo;
         for (int t = 0; t < steps; ++t) {
           const int T = step0 + t, buf = T & 1, I = 2 * T + side, at = I % L::NS;
           wait(&cfull[at], I / L::NS);
           const uint8_t *src = ring + at * L::CODE;
-          const uint16_t *scales = reinterpret_cast<const uint16_t *>(src + 64 * L::PITCH);
-          const int p0 = tile_of(u, t) * TP;
-          const bool part = p0 + TP > hi || (p0 < lo && p0 + TP > a.sinks);
           uint4 code[L::ITEMS];
           uint32_t by[L::ITEMS];
 #pragma unroll
           for (int i = 0; i < L::ITEMS; ++i) {
-            const int r = row_of(i), gr = group_of(i);
-            code[i] = *reinterpret_cast<const uint4 *>(src + pk_swz<L::PITCH>(r, gr));
-            by[i] = gr < chd ? scales[r * chd + gr] : 0u;
-            // a position no row sees counts as 0 whatever lies there
-            if (part && !(p0 + r < hi && (p0 + r >= lo || p0 + r < a.sinks))) by[i] = 0;
-            by[i] |= by[i] << 16;
+            const int down = i / ACROSS, over = i % ACROSS;  // over: 4 groups on, which an exclusive or does
+            code[i] = *reinterpret_cast<const uint4 *>(src + down * (DOWN * L::PITCH) + (src0 ^ (over * 64)));
+            by[i] = gr_l + L::LW * over < chd
+                        ? *reinterpret_cast<const uint16_t *>(src + sc0 + down * (DOWN * 2 * chd) + over * 2 * L::LW)
+                        : 0u;
           }
+          const int p0 = tile_of(u, t) * TP;
+          if (p0 + TP > hi || (p0 < lo && p0 + TP > a.sinks)) {
+            // a position no row sees counts as 0 whatever lies there
+#pragma unroll
+            for (int i = 0; i < L::ITEMS; ++i) {
+              const int p = p0 + r0 + (i / ACROSS) * DOWN;
+              if (!(p < hi && (p >= lo || p < a.sinks))) by[i] = 0;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < L::ITEMS; ++i) by[i] = __byte_perm(by[i], 0, 0x1010);
           __syncwarp();
           if (lane == 0) mbar_arrive(&cfree[at]);
           if (T >= 2) wait(&empty[side * 2 + buf], (T >> 1) - 1);
           uint8_t *dst = sm + (side * 2 + buf) * L::SIDE;
 #pragma unroll
           for (int i = 0; i < L::ITEMS; ++i) {
-            const int r = row_of(i), gr = group_of(i);
-            uint8_t *to = dst + (gr >> 1) * 8192 + r * 128;
             const uint32_t words[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t v[4];
               dequant_i4(words[k], v);
-              *reinterpret_cast<uint4 *>(to + ((((gr & 1) * 4 + k) ^ (r & 7)) << 4)) =
+              *reinterpret_cast<uint4 *>(dst + (dst0 ^ (k << 4)) + (i / ACROSS) * (DOWN * 128) + (i % ACROSS) * 16384) =
                   make_uint4(mul2(v[0], by[i]), mul2(v[1], by[i]), mul2(v[2], by[i]), mul2(v[3], by[i]));
             }
           }
