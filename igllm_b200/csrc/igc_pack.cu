@@ -738,10 +738,10 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 // ---------------------------------------------------------------------------
 // units cut between blocks, joined: block x takes the unit that attention
 // block x + 1 begins inside, if that is the unit's first cut.  `some` rows a
-// block, a row at a time by all its threads (a thread four columns of every
-// second, fourth or eighth piece of a narrow head) where there may be many
-// pieces, else a row by as many threads as it has fours of columns.  The order
-// of the additions is fixed.
+// block: one by all its threads (a thread four columns of every second, fourth
+// or eighth piece of a narrow head) where there may be many pieces, else each
+// by as many threads as it has fours of columns.  The order of the additions
+// is fixed.
 
 struct PackMerge {
   PackAttend a;
@@ -778,24 +778,35 @@ __global__ void __launch_bounds__(PM_THREADS) pack_merge_kernel(const __grid_con
     x.w = fmaf(y.w, f, x.w);
   };
   if (g.some > 1) {
-    for (int r = blockIdx.y * g.some + team; team < teams && r < (int)(blockIdx.y + 1) * g.some; r += teams) {
-      const int rr = c.b * RB + r;
-      if (rr >= c.q_n * a.group) break;
-      float m = -INFINITY, l = 0.0f;
-      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int i = 0; i < pieces; ++i) {
-        const float *p = at(i);
-        const float y = p[(size_t)RB * size + RB + r], ym = p[(size_t)RB * size + r];
-        const float4 v = *reinterpret_cast<const float4 *>(p + (size_t)r * size + col);
-        if (y == 0.0f) continue;  // it saw none of the row's positions
-        const float mx = fmaxf(m, ym), base = mx == -INFINITY ? 0.0f : mx, back = exp2_fast(m - base), f = exp2_fast(ym - base);
-        m = mx;
-        l = l * back + y * f;
-        x.x *= back, x.y *= back, x.z *= back, x.w *= back;
-        add(x, v, f);
+    const int r = blockIdx.y * g.some + team, rr = c.b * RB + r;
+    if (team >= g.some || rr >= c.q_n * a.group) return;
+    float m = -INFINITY, l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < pieces; i0 += 4) {
+      float ym[4], y[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = 0.0f;
+        if (i0 + i < pieces) {
+          const float *p = at(i0 + i);
+          y[i] = p[(size_t)RB * size + RB + r];
+          ym[i] = p[(size_t)RB * size + r];
+          v[i] = *reinterpret_cast<const float4 *>(p + (size_t)r * size + col);
+        }
       }
-      put(rr, x, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (y[i] == 0.0f) continue;  // it saw none of the row's positions
+        const float mx = fmaxf(m, ym[i]), base = mx == -INFINITY ? 0.0f : mx;
+        const float back = exp2_fast(m - base), f = exp2_fast(ym[i] - base);
+        m = mx;
+        l = l * back + y[i] * f;
+        x.x *= back, x.y *= back, x.z *= back, x.w *= back;
+        add(x, v[i], f);
+      }
     }
+    put(rr, x, l);
     return;
   }
   const int r = blockIdx.y, rr = c.b * RB + r;
@@ -1041,7 +1052,7 @@ cudaError_t igc_launch_pack_attend(const PackAttend *a, const PackPlan *p, cudaS
   e = p->tc ? igc_launch_pack_tc(a, p, &tmk, &tmv, st) : pack_run(*p, *a, tmk, tmv, st);
   if (e != cudaSuccess || p->grid == 1) return e;
   *launches = 2;
-  const int rb = 8 * p->rows8, some = p->tc ? 16 : 1;
+  const int rb = 8 * p->rows8, some = p->tc && PM_THREADS / (a->c.size / 4) >= 2 ? 2 : 1;
   const PackMerge g = {*a, rb, p->grid, some};
   return pack_launch(pack_merge_kernel, dim3((unsigned)p->grid - 1, rb / some), PM_THREADS, 0, st, true, g);
 }
