@@ -160,6 +160,7 @@ def _lib():
         "igc_model_device_bytes": (ctypes.c_size_t, [vp]),
         "igc_model_weight_count": (ctypes.c_size_t, [vp]),
         "igc_session_open": (i, [vp, _P(vp)]),
+        "igc_session_open_packed": (i, [vp, i, _P(vp)]),
         "igc_session_close": (None, [vp]),
         "igc_session_reset": (None, [vp]),
         "igc_session_hold": (i, [vp, i]),
@@ -227,7 +228,7 @@ def exported_symbols():
         "igc_back_open", "igc_back_close", "igc_desk_status", "igc_model_load", "igc_model_free",
         "igc_model_vocab_count", "igc_model_layer_count", "igc_model_state_size",
         "igc_model_window_limit", "igc_model_decode_bytes", "igc_model_device_bytes", "igc_model_weight_count",
-        "igc_session_open", "igc_session_close", "igc_session_reset", "igc_session_hold",
+        "igc_session_open", "igc_session_open_packed", "igc_session_close", "igc_session_reset", "igc_session_hold",
         "igc_session_prime", "igc_session_step", "igc_session_guess", "igc_session_guess_top",
         "igc_session_guess_keep", "igc_session_guess_taste", "igc_session_pick", "igc_session_fill",
         "igc_session_guess_span", "igc_session_guess_limit", "igc_session_round",
@@ -316,12 +317,19 @@ class Model:
 
 
 class Session:
-    """app_core.c:14219 session_open and the calls on a session."""
+    """app_core.c:14219 session_open and the calls on a session.  `packed` opens
+    one whose caches hold 4-bit codes (igc_session_open_packed), its sliding
+    layers keeping the first `sinks` positions in sight."""
 
-    def __init__(self, model):
+    def __init__(self, model, packed=False, sinks=0):
         self.model = model
         self._h = ctypes.c_void_p()
-        _check(_lib().igc_session_open(model._h, ctypes.byref(self._h)), "session_open")
+        if packed:
+            _check(_lib().igc_session_open_packed(model._h, int(sinks), ctypes.byref(self._h)), "session_open_packed")
+        elif sinks:
+            raise ValueError("Session: first positions stay in sight in packed sessions only")
+        else:
+            _check(_lib().igc_session_open(model._h, ctypes.byref(self._h)), "session_open")
 
     def close(self):
         if self._h:

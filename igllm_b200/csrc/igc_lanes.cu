@@ -701,6 +701,57 @@ __global__ void __launch_bounds__(256) lane_kv_kernel(const float *qkv, int qkv_
   }
 }
 
+// The same norms and turns for the packed cache, whose operators take plain
+// rows: a warp a head of the lane's queries, then (owner) of its new keys and
+// values.
+__global__ void __launch_bounds__(256) lane_turn_kernel(const float *qkv, int qkv_stride, int heads, int kv_heads,
+                                                        int hd, const float *q_norm, const float *k_norm,
+                                                        const float *cs_tab, const float *sn_tab, float eps,
+                                                        const int *p0, int owner, float *q_out, float *k_out,
+                                                        float *v_out, float *peak) {
+  pdl_release();
+  pdl_wait();
+  const int j = blockIdx.x, p = *p0 + j, half = hd / 2;
+  const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const float *cs = cs_tab + (size_t)p * half, *sn = sn_tab + (size_t)p * half;
+  for (int it = warp; it < heads + (owner ? 2 * kv_heads : 0); it += blockDim.x >> 5) {
+    const bool is_q = it < heads, is_v = it >= heads + kv_heads;
+    const float *src = qkv + (size_t)j * qkv_stride + (size_t)it * hd;  // heads, keys and values lie one after another
+    const float *gain = is_q ? q_norm : is_v ? nullptr : k_norm;
+    float *dst = is_q   ? q_out + ((size_t)j * heads + it) * hd
+                 : is_v ? v_out + ((size_t)j * kv_heads + it - heads - kv_heads) * hd
+                        : k_out + ((size_t)j * kv_heads + it - heads) * hd;
+    float lo[8], hi[8], ss = 0.0f, mx = 0.0f;  // heads up to 512: d = lane + 32 e < 256
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = l + 32 * e;
+      lo[e] = d < half ? src[d] : 0.0f;
+      hi[e] = d < half ? src[d + half] : 0.0f;
+      ss += lo[e] * lo[e] + hi[e] * hi[e];
+    }
+    const float sh = rms_shrink(warp_sum(ss), hd, eps);  // app_core.c:4667 kern_norm_rms
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = l + 32 * e;
+      if (d >= half) continue;
+      float x = lo[e] * sh, y = hi[e] * sh;
+      if (!is_v) {
+        x *= gain[d];
+        y *= gain[d + half];
+        const float c = cs[d], sv = sn[d];  // app_core.c:5196 kern_rope_turn: pairs (d, d + hd/2)
+        const float x2 = x * c - y * sv, y2 = y * c + x * sv;
+        x = x2;
+        y = y2;
+      }
+      mx = fmaxf(mx, fmaxf(fabsf(x), fabsf(y)));
+      dst[d] = x;
+      dst[d + half] = y;
+    }
+    mx = warp_max(mx);
+    if (!is_q && peak && l == 0) atomicMax(reinterpret_cast<int *>(peak) + (is_v ? 1 : 0), __float_as_int(mx));
+  }
+}
+
 // Rows of a layer's byte cache sides decoded into float rows the attention
 // kernel reads (app_core.c:11050 cache_grid_fill's table: each code's grid
 // value times the side's scale): block row z covers one session, rows [lo,
@@ -1073,6 +1124,15 @@ cudaError_t igc_launch_lane_kv_many(const float *qkv, int qkv_stride, int heads,
   KvTables tab = {pos_tab, kc_tab, vc_tab, peak_tab, per};
   return lane_launch(lane_kv_kernel, dim3(lanes), dim3(256), 0, st, qkv, qkv_stride, heads, kv_heads, hd, k_norm, cs,
                      sn, eps, p0, kc, vc, cq, tab);
+}
+
+cudaError_t igc_launch_lane_turn(const float *qkv, int qkv_stride, int heads, int kv_heads, int hd,
+                                 const float *q_norm, const float *k_norm, const float *cs, const float *sn, float eps,
+                                 const int *p0, int lanes, int owner, float *q_out, float *k_out, float *v_out,
+                                 float *peak, cudaStream_t st) {
+  if (lanes < 1 || hd < 2 || hd > 512 || hd % 2 || !q_norm || (owner && !k_norm)) return cudaErrorInvalidValue;
+  return lane_launch(lane_turn_kernel, dim3(lanes), dim3(256), 0, st, qkv, qkv_stride, heads, kv_heads, hd, q_norm,
+                     k_norm, cs, sn, eps, p0, owner, q_out, k_out, v_out, peak);
 }
 
 cudaError_t igc_launch_plain_product(const PlainArgs *a, int sm_count, int *blocks_out, cudaStream_t st) {

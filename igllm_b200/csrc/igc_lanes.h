@@ -135,6 +135,15 @@ cudaError_t igc_launch_lane_kv_many(const float *qkv, int qkv_stride, int heads,
                                     int lanes, float *kc, float *vc, const igc::CacheStore *store, const int *pos_tab,
                                     float *const *kc_tab, float *const *vc_tab, float *const *peak_tab, int per,
                                     cudaStream_t st);
+// A pass's `lanes` rows of q|k|v apart, ready for the packed cache's operators
+// (igc_pack.h): queries normed and turned into q_out [lane][heads][hd], and
+// with `owner` the new keys (normed and turned) and values (normed) into k_out
+// and v_out [lane][kv_heads][hd] and their largest magnitudes to peak [key,
+// value] (nullable).
+cudaError_t igc_launch_lane_turn(const float *qkv, int qkv_stride, int heads, int kv_heads, int hd,
+                                 const float *q_norm, const float *k_norm, const float *cs, const float *sn, float eps,
+                                 const int *p0, int lanes, int owner, float *q_out, float *k_out, float *v_out,
+                                 float *peak, cudaStream_t st);
 // Byte cache rows decoded into float rows for the attention kernel: for each
 // of `batch` sessions (tables) or one (pointers), rows [lo, p0 + lanes) of
 // each byte side (lo = p0 - span + 1 on a sliding layer, clipped at 0; 0 on

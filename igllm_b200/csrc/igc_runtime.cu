@@ -1097,6 +1097,15 @@ struct igc_session {
   // where a layer with a byte side has its rows decoded to floats for the
   // attention kernel (window x widest row floats a side; one layer at a time)
   float *kf = nullptr, *vf = nullptr;
+  // caches of 4-bit codes instead (igc_session_open_packed): per owner layer
+  // its codes and scales, one slot of the window rounded up to whole tiles;
+  // the first positions a sliding layer keeps in sight; a pass's turned rows
+  // and the attention's scratch, for `pack_lanes` lanes
+  bool packed = false;
+  int sinks = 0, pack_lanes = 0;
+  std::vector<PackView> pack;
+  float *pack_q = nullptr, *pack_k = nullptr, *pack_v = nullptr, *pack_work = nullptr;
+  size_t pack_work_floats = 0;
   // the first position whose rows every sliding layer holds: 0, except after
   // loading a file written from rings that had turned over
   int floor = 0;
@@ -1258,7 +1267,93 @@ static int widen_rows_most(const igc_model *m, int sliding, int lanes) {
   return r < m->window_limit ? r : m->window_limit;
 }
 
-extern "C" int igc_session_open(igc_model *m, igc_session **out) {
+// A packed session's attention of layer l over its owner's codes: plan for
+// `lanes` rows of one sequence.
+static cudaError_t pack_layer_plan(const igc_session *s, int l, int lanes, PackPlan *plan) {
+  const igc_model *m = s->m;
+  const DevLayer &L = m->layer[l], &O = m->layer[L.share ? L.source : l];
+  const PackView &view = s->pack[L.share ? L.source : l];
+  return igc_pack_plan(1, lanes, lanes, view.positions, O.kv_heads, m->heads / O.kv_heads, L.hd, 1,
+                       L.kind == 0 ? m->slide_span : 0, L.kind == 0 ? s->sinks : 0, plan);
+}
+
+// Room for packed passes of up to `lanes` lanes.
+static int pack_room(igc_session *s, int lanes) {
+  if (lanes <= s->pack_lanes) return IGC_OKAY;
+  const igc_model *m = s->m;
+  size_t work = 0, kv = 0;
+  for (int l = 0; l < m->layers; ++l) {
+    kv = std::max(kv, (size_t)m->layer[l].kv_rows);
+    bool seen = false;  // layers of one shape plan alike
+    for (int o = 0; o < l; ++o) seen = seen || (m->layer[o].hd == m->layer[l].hd && m->layer[o].kind == m->layer[l].kind);
+    for (int k = 1; k <= lanes && !seen; ++k) {
+      PackPlan plan;
+      CK(pack_layer_plan(s, l, k, &plan));
+      work = std::max(work, plan.work_floats);
+    }
+  }
+  int c = s->alloc(&s->pack_q, (size_t)lanes * m->max_q);
+  if (c == IGC_OKAY) c = s->alloc(&s->pack_k, (size_t)lanes * kv);
+  if (c == IGC_OKAY) c = s->alloc(&s->pack_v, (size_t)lanes * kv);
+  if (c == IGC_OKAY) c = s->alloc(&s->pack_work, work);
+  if (c != IGC_OKAY) return c;
+  s->pack_work_floats = work;
+  s->pack_lanes = lanes;
+  return IGC_OKAY;
+}
+
+// Layer l of a packed session's pass: queries turned, an owner's new rows
+// quantised into its cache, then attention over the codes, those rows' among
+// them, into `out`.
+static int pack_attend(igc_session *s, int l, const float *qkv, const int *p0, int lanes, float *out) {
+  const igc_model *m = s->m;
+  const DevLayer &L = m->layer[l];
+  const int owner = L.share ? L.source : l;
+  const DevLayer &O = m->layer[owner];
+  CKL(igc_launch_lane_turn(qkv, L.qkv_rows, m->heads, O.kv_heads, L.hd, L.q_norm, L.k_norm, m->rope_cs[L.kind],
+                           m->rope_sn[L.kind], m->eps, p0, lanes, L.share ? 0 : 1, s->pack_q, s->pack_k, s->pack_v,
+                           s->d_peak + 2 * owner, s->st));
+  const PackRows rows = {1, lanes, lanes, lanes, nullptr, p0, nullptr};
+  if (!L.share) {
+    const PackData k = {s->pack_k, 1, (long)O.kv_heads * L.hd, L.hd}, v = {s->pack_v, 1, (long)O.kv_heads * L.hd, L.hd};
+    CKL(igc_launch_pack_write(&s->pack[owner], &rows, &k, &v, s->st));
+  }
+  PackPlan plan;
+  CK(pack_layer_plan(s, l, lanes, &plan));
+  if (plan.work_floats > s->pack_work_floats) return IGC_FAIL_MEMORY;
+  const int group = m->heads / O.kv_heads, sliding = L.kind == 0;
+  const PackAttend a = {s->pack[owner],
+                        rows,
+                        {s->pack_q, 1, (long)m->heads * L.hd, L.hd},
+                        {out, 1, L.q_rows, L.hd},
+                        group,
+                        Quotient::by(group),
+                        sliding ? m->slide_span : 0,
+                        sliding ? s->sinks : 0,
+                        1.0f,  // app_core.c:11314: the norms carry the scale
+                        s->pack_work};
+  int launches = 0;
+  const cudaError_t e = igc_launch_pack_attend(&a, &plan, s->st, &launches);
+  g_launches += launches;
+  if (e != cudaSuccess) return fail_device(e, "igc_launch_pack_attend");
+  return IGC_OKAY;
+}
+
+static int session_open(igc_model *m, bool packed, int sinks, igc_session **out);
+
+extern "C" int igc_session_open(igc_model *m, igc_session **out) { return session_open(m, false, 0, out); }
+
+extern "C" int igc_session_open_packed(igc_model *m, int sinks, igc_session **out) {
+  if (!m || !out || sinks < 0) return IGC_FAIL_ARGUMENT;
+  *out = nullptr;
+  for (int l = 0; l < m->layers; ++l) {
+    const DevLayer &L = m->layer[l];
+    if (L.hd < PACK_GROUP || L.hd > 512 || L.hd % PACK_GROUP != 0) return IGC_FAIL_SUPPORT;
+  }
+  return session_open(m, true, sinks, out);
+}
+
+static int session_open(igc_model *m, bool packed, int sinks, igc_session **out) {
   if (!m || !out) return IGC_FAIL_ARGUMENT;
   *out = nullptr;
   clear_stale("session open");
@@ -1268,11 +1363,30 @@ extern "C" int igc_session_open(igc_model *m, igc_session **out) {
   CK(cudaStreamCreateWithFlags(&s->st, cudaStreamNonBlocking));
   const int K = IGC_LANE_LIMIT, H = m->hidden, PS = m->layers * m->ple_dim;
   int c = IGC_OKAY;
+  s->packed = packed;
+  s->sinks = sinks;
   s->kc.assign((size_t)m->layers, nullptr);
   s->vc.assign((size_t)m->layers, nullptr);
+  if (packed) s->pack.assign((size_t)m->layers, PackView{});
   for (int l = 0; l < m->layers && c == IGC_OKAY; ++l) {
     const DevLayer &L = m->layer[l];
     if (L.share) continue;
+    if (packed) {
+      PackView &p = s->pack[l];
+      p.slots = 1;
+      p.heads = L.kv_heads;
+      p.positions = (m->window_limit + PACK_TILE - 1) / PACK_TILE * PACK_TILE;
+      p.size = L.hd;
+      const size_t values = (size_t)p.positions * L.kv_rows;
+      c = s->alloc(&p.kc, values / 2);
+      if (c == IGC_OKAY) c = s->alloc(&p.vc, values / 2);
+      if (c == IGC_OKAY) c = s->alloc(&p.ks, values / PACK_GROUP);
+      if (c == IGC_OKAY) c = s->alloc(&p.vs, values / PACK_GROUP);
+      if (c != IGC_OKAY) break;
+      CK(cudaMemsetAsync(p.ks, 0, values / PACK_GROUP * 2, s->st));
+      CK(cudaMemsetAsync(p.vs, 0, values / PACK_GROUP * 2, s->st));
+      continue;
+    }
     const CacheStore cq = layer_store(m, l, nullptr);
     const size_t kb = side_bytes(cq.kq) * (size_t)m->window_limit * L.kv_rows;
     const size_t vb = side_bytes(cq.vq) * (size_t)m->window_limit * L.kv_rows;
@@ -1285,7 +1399,7 @@ extern "C" int igc_session_open(igc_model *m, igc_session **out) {
     CK(cudaMemsetAsync(kp, 0, kb, s->st));  // a zero code decodes to zero: a cleared cache either way
     CK(cudaMemsetAsync(vp, 0, vb, s->st));
   }
-  {
+  if (!packed) {
     int widest = 0;  // the widest row a byte side decodes into
     for (int l = 0; l < m->layers; ++l)
       if (!m->layer[l].share && layer_bytes(m, l)) widest = std::max(widest, m->layer[l].kv_rows);
@@ -1302,6 +1416,8 @@ extern "C" int igc_session_open(igc_model *m, igc_session **out) {
   if (c == IGC_OKAY) {
     s->d_err = s->d_top + K;
     CK(cudaMemsetAsync(s->d_top, 0, sizeof(int32_t) * (K + 1), s->st));
+    for (PackView &p : s->pack) p.trouble = s->d_err;
+    if (packed) c = pack_room(s.get(), K);
   }
   if (c == IGC_OKAY) c = s->alloc(&s->x0, (size_t)K * H);
   if (c == IGC_OKAY) c = s->alloc(&s->xa, (size_t)K * H);
@@ -1617,7 +1733,8 @@ static int enqueue_pass(igc_session *s, int K, int want) {
   // the one a two-pass prologue would find, so results do not depend on it
   const bool mags = true;
   Ssq *mact_out = mags ? &mact : nullptr, *mpa_out = mags ? &mpa : nullptr;
-  const Ssq *ma_in = mags ? &ma : nullptr, *mact_in = mags ? &mact : nullptr, *mpa_in = mags ? &mpa : nullptr;
+  // (a packed session's attention leaves none)
+  const Ssq *ma_in = mags && !s->packed ? &ma : nullptr, *mact_in = mags ? &mact : nullptr, *mpa_in = mags ? &mpa : nullptr;
   const Ssq *pend_ssq = nullptr;
   auto next_x = [&]() -> float * { float *o = bufs[flip]; flip ^= 1; return o; };
   for (int l = 0; l < m->layers; ++l) {
@@ -1638,7 +1755,10 @@ static int enqueue_pass(igc_session *s, int K, int want) {
     const DevLayer &O = m->layer[owner];
     prof_mark(s, PROF_ATTN, 0.0);
     const int sliding = L.kind == 0 ? 1 : 0;
-    if (!layer_split(m, l)) {
+    if (s->packed) {
+      c = pack_attend(s, l, s->qkv, d_p0, K, s->attn);
+      if (c != IGC_OKAY) return c;
+    } else if (!layer_split(m, l)) {
       // queries, an owner's new rows and the attention in one kernel
       const CacheStore cq = layer_store(m, owner, L.share ? nullptr : s->d_peak + 2 * l);
       CKL(igc_launch_attn(s->qkv, L.qkv_rows, m->heads, O.kv_heads, L.hd, L.q_norm, L.k_norm, m->rope_cs[L.kind],
@@ -2064,7 +2184,8 @@ static int chunks_ready(igc_session *s) {
   if (C.B.cap) return IGC_OKAY;
   const int M = chunk_lanes();
   igc_model *m = s->m;
-  int c = lane_buf_alloc(m, C.B, M, 0, s->owned);
+  int c = s->packed ? pack_room(s, M) : IGC_OKAY;
+  if (c == IGC_OKAY) c = lane_buf_alloc(m, C.B, M, 0, s->owned);
   C.groups_cap = M / 16 + 1;
   if (c == IGC_OKAY) c = s->alloc(&C.d_ids, 1 + M);
   if (c == IGC_OKAY) c = s->alloc(&C.d_pos, C.groups_cap);
@@ -2104,6 +2225,7 @@ static int enqueue_chunk(igc_session *s, int M, bool head, bool want) {
   // without overlap: a group copies cached rows before its own wait, and
   // those rows are the prep launch's writes.
   auto attend = [&](int l, const DevLayer &L) -> int {
+    if (s->packed) return pack_attend(s, l, C.B.qkv, C.d_ids, M, C.B.attn);
     const int owner = L.share ? L.source : l;
     const DevLayer &O = m->layer[owner];
     const int full = M / 16, tail = M - 16 * full, sliding = L.kind == 0 ? 1 : 0;
@@ -2417,7 +2539,11 @@ extern "C" size_t igc_session_cache_room_at(const igc_session *s, int cache_bits
   return total;
 }
 extern "C" size_t igc_session_cache_room(const igc_session *s) {
-  return s ? igc_session_cache_room_at(s, s->m->cache_bits) : 0;
+  if (!s || !s->packed) return s ? igc_session_cache_room_at(s, s->m->cache_bits) : 0;
+  size_t total = 0;
+  for (const PackView &p : s->pack)
+    total += (size_t)p.heads * p.positions * 2 * (p.size / 2 + p.size / PACK_GROUP * 2);
+  return total;
 }
 
 extern "C" int igc_session_ids(const igc_session *s, int32_t *ids, int limit) { /* app_core.c:14183 */
@@ -2441,6 +2567,7 @@ extern "C" int igc_session_save(const igc_session *s, const char *path, uint64_t
                                 int kind) { /* app_core.c:14010 */
   if (!s || !path) return IGC_FAIL_ARGUMENT;
   if (s->guess_count > 0) return IGC_FAIL_STATE;
+  if (s->packed) return IGC_FAIL_SUPPORT;  // the reference's file holds floats or e4m3 bytes
   if (kind != IGC_KEEP_PROMPT && kind != IGC_KEEP_TALK) return IGC_FAIL_ARGUMENT;
   const igc_model *m = s->m;
   if (note && !note_sane(note, m->window_limit)) return IGC_FAIL_ARGUMENT;
@@ -2502,6 +2629,7 @@ extern "C" int igc_session_load(igc_session *s, const char *path, uint64_t *stam
                                 int *kind_out) { /* app_core.c:14076 */
   if (!s || !path) return IGC_FAIL_ARGUMENT;
   if (s->guess_count > 0) return IGC_FAIL_STATE;
+  if (s->packed) return IGC_FAIL_SUPPORT;
   if (stamp_out) *stamp_out = 0;
   if (kind_out) *kind_out = IGC_KEEP_PROMPT;
   if (note_out) memset(note_out, 0, sizeof(*note_out));
@@ -2754,6 +2882,7 @@ extern "C" int igc_crowd_round(igc_crowd *cr, igc_session **sessions, int count,
   for (int j = 0; j < count; ++j) {
     igc_session *s = sessions[j];
     if (!s || s->m != m) return IGC_FAIL_ARGUMENT;
+    if (s->packed) return IGC_FAIL_SUPPORT;
     if (s->guess_count > 0) return IGC_FAIL_STATE;
     if (s->fill + k > m->window_limit) return IGC_FAIL_STATE;
     for (int q = 0; q < j; ++q)

@@ -154,6 +154,15 @@ size_t igc_model_weight_count(const igc_model *model);
 
 /* app_core.c:14219 session_open / :14368 session_close / :14375 session_reset */
 int igc_session_open(igc_model *model, igc_session **session_out);
+/* A session whose caches hold 4-bit codes (the packed cache of part 3), 0.5625
+ * bytes a value against a float cache's 4 (no counterpart in the reference).
+ * Its passes write their rows as codes and attend over the codes, those rows'
+ * among them; its sliding layers keep the first `sink_count` positions in
+ * sight beside their window (0: the window alone, as the reference).  Every
+ * call on a session works on it but igc_session_save, igc_session_load and
+ * igc_crowd_round, which refuse it with IGC_FAIL_SUPPORT, as the open refuses
+ * a model with a head that is not a multiple of 32 wide. */
+int igc_session_open_packed(igc_model *model, int sink_count, igc_session **session_out);
 void igc_session_close(igc_session *session);
 void igc_session_reset(igc_session *session);
 /* app_core.c:13935 session_hold.  Caches are full length, so no ring turns

@@ -194,6 +194,7 @@ struct igo_session {
   int echo_count, echo_limit;
   int guess_count, guess_from, guess_echo;
   uint64_t draw_state;
+  int packed, sinks, doubts;  /* igo_session_pack */
   /* lane rooms */
   float *x, *h, *q, *k, *v, *blend, *lift, *gate, *up, *ple, *seed, *score, *cs, *sn;
 };
@@ -249,6 +250,49 @@ void igo_session_close(igo_session *s) {
 
 int igo_session_fill(const igo_session *s) { return s->fill; }
 
+void igo_session_pack(igo_session *s, int sinks) {
+  s->packed = 1;
+  s->sinks = sinks;
+}
+
+int igo_session_doubts(igo_session *s) {
+  int n = s->doubts;
+  s->doubts = 0;
+  return n;
+}
+
+/* A float to the nearest half, ties to even, as a float (positive, below
+ * 65504; below 2^-14 the steps are 2^-24). */
+static float half_of(float x) {
+  int e = 0;
+  if (x <= 0.0f) return 0.0f;
+  frexpf(x, &e); /* x in [2^(e-1), 2^e): 11 significant bits are steps of 2^(e-11) */
+  if (e < -13) e = -13;
+  return ldexpf(rintf(ldexpf(x, 11 - e)), e - 11);
+}
+
+/* What a row becomes in the packed cache: per 32 columns a half scale of the
+ * largest magnitude over 7, and whole numbers of it in [-8, 7].  Returns the
+ * groups whose choices are near a tie. */
+static int pack_row(float *x, int n) {
+  const float near = 4e-6f; /* of a value: the two sides' rows differ by about 1e-6 */
+  int doubts = 0;
+  for (int g = 0; g < n; g += 32) {
+    float big = 0.0f, step;
+    int doubt;
+    for (int i = 0; i < 32; ++i) big = fmaxf(big, fabsf(x[g + i]));
+    step = half_of(fminf(big / 7.0f, 8188.0f));
+    doubt = half_of(big / 7.0f * (1.0f - near)) != half_of(big / 7.0f * (1.0f + near));
+    for (int i = 0; i < 32; ++i) {
+      float r = step > 0.0f ? x[g + i] / step : 0.0f, q = rintf(r);
+      doubt |= rintf(r - 8.0f * near) != rintf(r + 8.0f * near);
+      x[g + i] = fminf(fmaxf(q, -8.0f), 7.0f) * step;
+    }
+    doubts += doubt;
+  }
+  return doubts;
+}
+
 int igo_session_echo(const igo_session *s, int32_t *out, int limit) {
   int n = s->echo_count < limit ? s->echo_count : limit;
   memcpy(out, s->echo, sizeof(int32_t) * (size_t)n);
@@ -303,6 +347,9 @@ static void attend(igo_session *s, int li, int place_from, int lanes, const floa
         igo_rope_turn(kk, hd, s->cs, s->sn);
         igo_norm_rms(vv, NULL, hd, m->eps, vv);
       }
+      if (s->packed) {
+        s->doubts += pack_row(kl, kvw) + pack_row(vl, kvw);
+      }
       memcpy(s->kc[li] + (size_t)place * kvw, kl, sizeof(float) * (size_t)kvw);
       memcpy(s->vc[li] + (size_t)place * kvw, vl, sizeof(float) * (size_t)kvw);
     }
@@ -312,10 +359,12 @@ static void attend(igo_session *s, int li, int place_from, int lanes, const floa
     }
     for (int hh = 0; hh < m->heads; ++hh) {
       const float *qh = ql + (size_t)hh * hd;
-      int kvh = hh / group, span = place - start + 1;
+      /* the first positions in sight, then the window's */
+      int kvh = hh / group, first = s->sinks < start ? s->sinks : start, span = first + place - start + 1;
       float *bh = bl + (size_t)hh * hd;
       for (int i = 0; i < span; ++i) {
-        const float *kr = s->kc[owner] + (size_t)(start + i) * kvw + (size_t)kvh * hd;
+        int at = i < first ? i : start + i - first;
+        const float *kr = s->kc[owner] + (size_t)at * kvw + (size_t)kvh * hd;
         float t = 0.0f;
         for (int d = 0; d < hd; ++d) t += kr[d] * qh[d];
         s->score[i] = t; /* score scale is 1.0 (app_core.c:11314) */
@@ -323,7 +372,8 @@ static void attend(igo_session *s, int li, int place_from, int lanes, const floa
       igo_soft_max(s->score, span);
       for (int d = 0; d < hd; ++d) bh[d] = 0.0f;
       for (int i = 0; i < span; ++i) {
-        const float *vr = s->vc[owner] + (size_t)(start + i) * kvw + (size_t)kvh * hd;
+        int at = i < first ? i : start + i - first;
+        const float *vr = s->vc[owner] + (size_t)at * kvw + (size_t)kvh * hd;
         float wgt = s->score[i];
         for (int d = 0; d < hd; ++d) bh[d] += wgt * vr[d];
       }

@@ -76,6 +76,12 @@ typedef struct igo_session igo_session;
 
 igo_session *igo_session_open(const igo_model *model, int threads);
 void igo_session_close(igo_session *s);
+/* From here on rows enter the caches as the packed cache's 4-bit groups hold
+ * them, and sliding layers also see the first `sinks` positions. */
+void igo_session_pack(igo_session *s, int sinks);
+/* How many groups came so near a rounding tie, of their scale or of a code,
+ * that another order of sums may store them otherwise; counts from 0 again. */
+int igo_session_doubts(igo_session *s);
 int igo_session_fill(const igo_session *s);
 /* app_core.c:14443 session_prime: every id but the last, 16 lanes a pass */
 int igo_session_prime(igo_session *s, const int32_t *ids, int n);

@@ -125,6 +125,8 @@ def igo_lib():
         i32p = ctypes.POINTER(ctypes.c_int32)
         for name, res, args in [
             ("igo_session_open", vp, [ctypes.POINTER(IgoModel), i]),
+            ("igo_session_pack", None, [vp, i]),
+            ("igo_session_doubts", i, [vp]),
             ("igo_session_close", None, [vp]),
             ("igo_session_fill", i, [vp]),
             ("igo_session_prime", i, [vp, i32p, i]),
@@ -291,10 +293,12 @@ class OracleModel:
 class OracleSession:
     """app_core.c session API over the restatement."""
 
-    def __init__(self, model, threads=8):
+    def __init__(self, model, threads=8, packed=False, sinks=0):
         self.model = model
         self.lib = igo_lib()
         self.h = self.lib.igo_session_open(ctypes.byref(model.m), threads)
+        if packed:
+            self.lib.igo_session_pack(self.h, int(sinks))
 
     def close(self):
         if self.h:
@@ -325,6 +329,9 @@ class OracleSession:
 
     def guess_keep(self, keep):
         return self.lib.igo_session_guess_keep(self.h, int(keep))
+
+    def doubts(self):
+        return self.lib.igo_session_doubts(self.h)
 
     def hold(self, keep):
         return self.lib.igo_session_hold(self.h, int(keep))

@@ -98,3 +98,10 @@ def test_a_cache_is_made_of_cuda_tensors(igc_lib):
         igc_lib.PackCache(codes, scales.float(), codes, scales)
     with pytest.raises(ValueError):
         igc_lib.PackCache(codes[0], scales, codes, scales)
+
+
+def test_packed_session_refuses_bad_arguments(igc_lib):
+    lib, out = igc_lib._lib(), ctypes.c_void_p(1)
+    assert lib.igc_session_open_packed(None, 0, ctypes.byref(out)) == igc_lib.FAIL_ARGUMENT
+    assert lib.igc_session_open_packed(None, -1, ctypes.byref(out)) == igc_lib.FAIL_ARGUMENT
+    assert lib.igc_session_open_packed(None, 0, None) == igc_lib.FAIL_ARGUMENT
