@@ -42,6 +42,10 @@ struct PackTc {
   static constexpr int SB = 4;
   static constexpr int PITCH = HDP / 2 < 128 ? HDP / 2 : 128;  // code bytes of a row
   static constexpr int NS = HDP == 256 ? 3 : 6;         // codes in flight: a side of a tile a place
+  // Barriers that codes are there, one a side even where the sides take a
+  // place in turns: a warp that waits for a phase has to have seen the phase
+  // before it complete, which it knows of its own side's only.
+  static constexpr int NF = NS % 2 ? 2 * NS : NS;
   static constexpr int CODE = 64 * PITCH + 64 * C * 2;  // codes, then scales
   static constexpr int OFF_Q = 4 * SIDE;                // the queries, 16 KB a 64-column block
   static constexpr int OFF_CODE = OFF_Q + BLOCKS * RB * 128;
@@ -188,23 +192,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   using L = PackTc<HDP>;
   constexpr int RB = L::RB, TP = L::TP, C = L::C;
   extern __shared__ __align__(1024) uint8_t tc_raw[];
-  __shared__ uint64_t bars[28 + 2 * L::NS];
+  __shared__ uint64_t bars[30 + L::NF + L::NS];
   __shared__ uint32_t tmem_slot;
   __shared__ float shared_m[2][RB], half_big[2][RB], half_sum[2][RB];
   __shared__ TcUnit units[2];
   uint8_t *sm = tc_raw + ((1024 - (smem_u32(tc_raw) & 1023)) & 1023);
   // [side][buffer] filled by the code warps, and free again; [score place]
   // scores ready, weights ready, values added; maxima told; queries ready; a
-  // unit told, and done with; [place] codes there, and free again
+  // unit told, and done with; the last product over; the softmax warps' halves
+  // of a row told (maxima, sums); codes there; [place] free again
   uint64_t *full = bars, *empty = bars + 4, *sfull = bars + 8, *pfull = bars + 12, *vdone = bars + 16, *mtold = bars + 20,
-           *qfull = bars + 22, *told = bars + 23, *done = bars + 25, *cfull = bars + 28, *cfree = cfull + L::NS;
+           *qfull = bars + 22, *told = bars + 23, *done = bars + 25, *over = bars + 27, *both = bars + 28, *cfull = bars + 30,
+           *cfree = cfull + L::NF;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
     for (int i = 0; i < L::SB; ++i) mbar_init(&sfull[i], 1), mbar_init(&pfull[i], 128), mbar_init(&vdone[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&mtold[i], 128), mbar_init(&told[i], 1), mbar_init(&done[i], 17);
     mbar_init(qfull, 256);
-    for (int i = 0; i < L::NS; ++i) mbar_init(&cfull[i], 1), mbar_init(&cfree[i], 4);
+    mbar_init(over, 1);
+    mbar_init(&both[0], 256), mbar_init(&both[1], 256);
+    for (int i = 0; i < L::NF; ++i) mbar_init(&cfull[i], 1);
+    for (int i = 0; i < L::NS; ++i) mbar_init(&cfree[i], 4);
     mbar_init_fence();
   }
   if (warp == 16) {
@@ -221,7 +230,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   int step0 = 0;                 // steps before this unit
   auto wait = [&](uint64_t *bar, int phase) {
     if (!mbar_wait(bar, (uint32_t)(phase & 1), failed ? PACK_TRIES / 64 : PACK_TRIES)) failed = true;
-    __syncwarp();  // lanes may leave the polls apart, and what follows takes the warp as one
+    // the warp as one: lanes may leave the polls apart
+    failed = __any_sync(0xffffffffu, failed);
   };
   auto tile_of = [](const TcUnit &u, int t) {
     const int k = u.ka + t;
@@ -234,7 +244,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const bool one = elect_one();
     const uint64_t policy = tall ? l2_evict_last() : l2_evict_first();  // other blocks of a prompt read them too
     PackWalk w;
-    int share;
+    int share, issued = 0;  // copies of a side of a tile
     bool any = walk_start<RB, TP, L::OVER>(a, tall, w, &share);
     if (one) leave_cut(a, w, any);
     for (int u = 0;; ++u) {
@@ -266,18 +276,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       __syncwarp();
       if (steps < 0 || failed) break;
-      for (int t = 0; t < steps; ++t) {
+      for (int t = 0; t < steps && !failed; ++t) {
         const int p0 = base + w.sp.tile(w.ka + t) * TP;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
           const int I = 2 * (step0 + t) + side, at = I % L::NS;
           if (I >= L::NS) wait(&cfree[at], I / L::NS - 1);
+          if (failed) break;  // the place may be in use
+          issued = I + 1;
           if (one) {
             uint8_t *dst = sm + L::OFF_CODE + at * L::CODE;
-            mbar_expect(&cfull[at], (uint32_t)(64 * L::PITCH + 64 * chd * 2));
-            pk_load(dst, side ? &tmv : &tmk, 0, p0, &cfull[at]);
+            uint64_t *there = &cfull[I % L::NF];
+            mbar_expect(there, (uint32_t)(64 * L::PITCH + 64 * chd * 2));
+            pk_load(dst, side ? &tmv : &tmk, 0, p0, there);
             bulk_load(dst + 64 * L::PITCH, (side ? a.c.vs : a.c.ks) + (size_t)p0 * chd, (uint32_t)(64 * chd * 2),
-                      &cfull[at], policy);
+                      there, policy);
           }
           __syncwarp();
         }
@@ -285,6 +298,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       step0 += steps;
       any = walk_next<RB, TP, L::OVER>(a, w, share);
     }
+    // no copy is under way when the block ends, whatever ended it
+    for (int I = max(0, issued - L::NS); I < issued; ++I) wait(&cfull[I % L::NF], I / L::NF);
   } else {
     int spent = 0;  // units that had steps
     for (int un = 0;; ++un) {
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         const int hi = u.hi, lo = u.lo;
         for (int t = 0; t < steps; ++t) {
           const int T = step0 + t, buf = T & 1, I = 2 * T + side, at = I % L::NS;
-          wait(&cfull[at], I / L::NS);
+          wait(&cfull[I % L::NF], I / L::NF);
           const uint8_t *src = ring + at * L::CODE;
           uint4 code[L::ITEMS];
           uint32_t by[L::ITEMS];
@@ -393,6 +408,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         constexpr int PIECES = HDP / 16, AT_ONCE = 32 / PIECES;
         auto row_at = [&](long at, int i) { return __shfl_sync(0xffffffffu, at, i * AT_ONCE + lane / PIECES); };
         const int my_piece = lane % PIECES, my_col = half * (HDP / 2) + 8 * my_piece;
+        auto meet = [&](int i) {
+          mbar_arrive(&both[i]);
+          wait(&both[i], un);
+        };
         float f = 0.0f;
         if (steps > 0) {
           const bool wide = wide_rows(a.q), bf = a.q.type == 3;
@@ -437,7 +456,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
           }
           half_big[half][r] = big;
-          named_sync(1, 256);
+          meet(0);
           big = __uint_as_float(max(__float_as_uint(big), __float_as_uint(half_big[half ^ 1][r])));
           // bf16: by the power of two that puts the largest in [2^13, 2^14); f16: as they are.  The
           // scale's sign goes along, so that the largest score is the largest weight's.
@@ -460,7 +479,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           fence_async_smem();
           mbar_arrive(qfull);
         } else {
-          named_sync(1, 256);  // the sums of the unit before are read
+          meet(0);  // the sums of the unit before are read
         }
         const int p_row = u.fill + token, pos = live && p_row < a.c.positions ? max(p_row, -1) : -1;
         const int p_first = u.fill + a.by_group.of(u.rr0), p_last = u.hi - 1, past = u.past;
@@ -573,7 +592,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           tc_after();
         }
         half_sum[half][r] = l;
-        named_sync(1, 256);
+        meet(1);
         l += half_sum[half ^ 1][r];
         if (!idle) {
           const bool wide = wide_rows(a.out), whole = u.whole;
@@ -650,6 +669,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       spent += steps > 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[un & 1]);
+    }
+    if (warp == 16) {  // nor is a product, or an arrival on a barrier
+      if (elect_one()) tc_commit(over);
+      wait(over, 0);
     }
   }
   if (failed) pack_trouble(a.c);
