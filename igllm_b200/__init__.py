@@ -672,6 +672,9 @@ class PackCache:
         self._index = self.device.index
         self._int32 = torch.int32
         self._raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, no object made
+        self._empty_like = torch.empty_like
+        lib = _lib()
+        self._write, self._read, self._attend = lib.igc_pack_write, lib.igc_pack_read, lib.igc_pack_attend
         self._room = {}  # scratch bytes by a call's sizes
         if positions % PACK_TILE or self.size % PACK_GROUP or not PACK_GROUP <= self.size <= 512:
             raise ValueError(f"PackCache: {positions} positions (a multiple of {PACK_TILE}) of {self.size} values "
@@ -692,49 +695,54 @@ class PackCache:
 
         return cls(codes(), scales(), codes(), scales())
 
+    # A small call's time is this side's: what follows reads each tensor's
+    # attributes once and makes no objects beside the arguments (attention of one
+    # token 15.5 us a call before, 5.5 of them below the binding).
+
     def _list(self, t, name, n):
-        if t is None:
-            return None
-        if t.dtype is not self._int32 or t.shape != (n,) or t.device != self.device or (n > 1 and t.stride(0) != 1):
+        if t.dtype is not self._int32 or t.dim() != 1 or t.numel() != n or t.get_device() != self._index or \
+                not t.is_contiguous():
             raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not {n} int32 on "
                              f"{self.device}")
         return t.data_ptr()
 
     def _rows(self, rows, fill, starts, slots, rows_most):
-        n = fill.shape[0]
-        return IgcPackRows(n, rows, 0 if rows_most is None else int(rows_most), self._list(starts, "starts", n + 1),
-                           self._list(fill, "fill", n), self._list(slots, "slots", n))
+        n = fill.numel()
+        return IgcPackRows(n, rows, rows_most or 0, None if starts is None else self._list(starts, "starts", n + 1),
+                           self._list(fill, "fill", n), None if slots is None else self._list(slots, "slots", n))
 
     def _data(self, t, name, rows, heads):
-        if t.shape != (rows, heads, self.size) or t.device != self.device or t.dtype not in self._types:
+        kind, stride = self._types.get(t.dtype), t.stride()
+        if kind is None or t.get_device() != self._index or t.shape != (rows, heads, self.size):
             raise ValueError(f"PackCache: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, not rows of "
                              f"{(rows, heads, self.size)} on {self.device}")
-        row, head, last = t.stride()
-        if last != 1 and t.numel():
+        if stride[2] != 1 and t.numel():
             raise ValueError(f"PackCache: the values of a head of {name} are not adjacent")
-        return IgcPackData(t.data_ptr(), self._types[t.dtype], row, head)
-
-    def _stream(self):
-        return self._raw_stream(self._index)
+        return IgcPackData(t.data_ptr(), kind, stride[0], stride[1])
 
     def write(self, keys, values, fill, starts=None, slots=None, rows_most=None):
         """Rows [n, heads, size] quantised into their places."""
         n = keys.shape[0]
         if n == 0:
             return
-        _check(_lib().igc_pack_write(self._p, self._rows(n, fill, starts, slots, rows_most),
-                                     self._data(keys, "keys", n, self.heads),
-                                     self._data(values, "values", n, self.heads), self._stream()), "pack_write")
+        code = self._write(self._p, self._rows(n, fill, starts, slots, rows_most),
+                           self._data(keys, "keys", n, self.heads), self._data(values, "values", n, self.heads),
+                           self._raw_stream(self._index))
+        if code:
+            raise IgcError(code, "pack_write")
 
     def read(self, fill, rows, dtype, starts=None, slots=None, rows_most=None, out=None):
         """(keys, values) of `rows` rows decoded, [rows, heads, size] of `dtype`
         (in arrays made here, rows of no sequence hold nothing of meaning)."""
         if out is None:
-            out = fill.new_empty((2, rows, self.heads, self.size), dtype=dtype).unbind(0)
+            keys = fill.new_empty((rows, self.heads, self.size), dtype=dtype)
+            out = keys, self._empty_like(keys)
         if rows:
-            _check(_lib().igc_pack_read(self._p, self._rows(rows, fill, starts, slots, rows_most),
-                                        self._data(out[0], "keys", rows, self.heads),
-                                        self._data(out[1], "values", rows, self.heads), self._stream()), "pack_read")
+            code = self._read(self._p, self._rows(rows, fill, starts, slots, rows_most),
+                              self._data(out[0], "keys", rows, self.heads),
+                              self._data(out[1], "values", rows, self.heads), self._raw_stream(self._index))
+            if code:
+                raise IgcError(code, "pack_read")
         return out
 
     def attend(self, queries, fill, starts=None, slots=None, window=0, sinks=0, scale=1.0, rows_most=None, out=None):
@@ -742,13 +750,13 @@ class PackCache:
         a sequence, at fill + i, sees every position up to its own, with a window
         only the last `window` of them and the first `sinks` of all."""
         n, heads = queries.shape[0], queries.shape[1]
-        if out is None:
-            out = queries.new_empty(queries.shape)
+        if out is None:  # contiguous, whatever the queries' strides
+            out = self._empty_like(queries) if queries.is_contiguous() else queries.new_empty(queries.shape)
         if n == 0:
             return out
         rows = self._rows(n, fill, starts, slots, rows_most)
         q, o = self._data(queries, "queries", n, heads), self._data(out, "out", n, heads)
-        key = (n, rows.count, rows.rows_most, starts is None, heads, q.real_type, window, sinks)
+        key = (n, fill.numel(), rows_most, starts is None, heads, queries.dtype, window, sinks)
         room = self._room.get(key)
         if room is None:
             need = ctypes.c_size_t()
@@ -758,14 +766,16 @@ class PackCache:
                 self._room.clear()
             room = self._room[key] = need.value
         work = self.key_codes.new_empty(room) if room else None
-        _check(_lib().igc_pack_attend(self._p, rows, heads, q, o, window, sinks, scale,
-                                      work.data_ptr() if room else None, room, self._stream()), "pack_attend")
+        code = self._attend(self._p, rows, heads, q, o, window, sinks, scale, work.data_ptr() if room else None, room,
+                            self._raw_stream(self._index))
+        if code:
+            raise IgcError(code, "pack_attend")
         return out
 
     def status(self):
         """Waits for the current stream; raises IgcError (FAIL_STATE) where a call
         since the last status met rows that do not fit the cache."""
-        _check(_lib().igc_pack_status(self._p, self._stream()), "pack_status")
+        _check(_lib().igc_pack_status(self._p, self._raw_stream(self._index)), "pack_status")
 
 
 def synth_write(spec, folder, threads=8):
