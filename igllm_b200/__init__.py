@@ -643,7 +643,8 @@ class PackCache:
     None for the sequence's own number; `rows_most` the most rows of any
     sequence (None: all rows).  These are CUDA tensors that the kernels read.
     Rows of no sequence are left as they are, rows at negative positions are
-    padding, and what does not fit the cache is left out and told by status()."""
+    padding, and what does not fit the cache is left out and told by status().
+    Nothing here is differentiated."""
 
     def __init__(self, key_codes, key_scales, value_codes, value_scales):
         import torch

@@ -3438,7 +3438,7 @@ bool pack_sane(const igc_pack *p) {
     return false;
   if (p->head_size < PACK_GROUP || p->head_size > 512 || p->head_size % PACK_GROUP != 0) return false;
   if (p->device < 0 || p->head_count > 32767) return false;
-  return (double)p->slot_count * p->head_count * p->position_count < 2147483648.0;  // positions are counted in ints
+  return (double)p->slot_count * p->head_count * p->position_count <= 1073741824.0;  // positions are counted in ints
 }
 
 bool pack_rows_sane(const igc_pack *p, const igc_pack_rows *r) {
@@ -3452,6 +3452,14 @@ bool pack_data_sane(const igc_pack_data *d) {
   if (!d || !d->data || d->real_type < 1 || d->real_type > 3) return false;
   if ((size_t)d->data % (d->real_type == 1 ? 4 : 2) != 0) return false;
   return d->row_stride >= 0 && d->head_stride >= 0;
+}
+
+// An array that a call writes: no two of its heads' values in one place.
+bool pack_apart(const igc_pack_data *d, int rows, int heads, int size) {
+  const double r = (double)d->row_stride, h = (double)d->head_stride;
+  if (rows > 1 && r < size) return false;
+  if (heads > 1 && h < size) return false;
+  return rows < 2 || heads < 2 || r >= (heads - 1) * h + size || h >= (rows - 1) * r + size;
 }
 
 PackView pack_view(const igc_pack *p) {
@@ -3476,6 +3484,9 @@ int pack_move(bool write, const igc_pack *p, const igc_pack_rows *rows, const ig
   if (!pack_sane(p) || !pack_rows_sane(p, rows) || !pack_data_sane(k) || !pack_data_sane(v)) return IGC_FAIL_ARGUMENT;
   if (k->real_type != v->real_type) return IGC_FAIL_ARGUMENT;
   if (rows->row_count == 0) return IGC_OKAY;
+  if (!write && (!pack_apart(k, rows->row_count, p->head_count, p->head_size) ||
+                 !pack_apart(v, rows->row_count, p->head_count, p->head_size)))
+    return IGC_FAIL_ARGUMENT;
   clear_stale("pack rows");
   DeviceScope dev(p->device);
   if (int c = dev.enter()) return c;
@@ -3531,6 +3542,7 @@ extern "C" int igc_pack_attend(const igc_pack *p, const igc_pack_rows *rows, int
     return IGC_FAIL_ARGUMENT;
   if (q->real_type != out->real_type || !std::isfinite(scale) || ((size_t)work & 15) != 0) return IGC_FAIL_ARGUMENT;
   if (rows->row_count == 0) return IGC_OKAY;
+  if (!pack_apart(out, rows->row_count, heads, p->head_size)) return IGC_FAIL_ARGUMENT;
   clear_stale("pack attend");
   DeviceScope dev(p->device);
   if (int c = dev.enter()) return c;

@@ -361,8 +361,8 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * is stored as 0.  Codes are [slot][head][position][head_size / 2] bytes,
  * scales [slot][head][position][head_size / 32] halves, keys and values apart,
  * each array on a 16-byte boundary; `position_count` is a multiple of 64 and
- * `head_size` of 32, at most 512; slots, heads and positions multiply to less
- * than 2^31.  `trouble`, when not NULL, is a device word
+ * `head_size` of 32, at most 512; there are at most 32767 heads, and slots,
+ * heads and positions multiply to at most 2^30.  `trouble`, when not NULL, is a device word
  * (zero at first) that calls set where what they find on the device does not
  * fit the cache; igc_pack_status reads and clears it.
  *
@@ -379,7 +379,8 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * places written by one call are the caller's to keep distinct.
  *
  * igc_pack_data is an array of rows: `real_type` 1 F32, 2 F16, 3 BF16 (the
- * reference's store_type values), strides in values, a head's values adjacent.
+ * reference's store_type values), strides in values, a head's values adjacent;
+ * in an array that a call writes no two heads' values share a place.
  *
  * igc_pack_write: keys and values (row_count x head_count x head_size, of one
  * type) into their places.  igc_pack_read: the same places decoded.

@@ -470,3 +470,80 @@ def test_refusals_leave_everything_alone(igc_lib):
     assert torch.equal(s.cache.key_codes, codes)
     s.cache.status()
     assert s.cache.attend(s.q[:0], s.fills, starts=torch.zeros_like(s.starts)).shape == (0, 8, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,size", [(71, 1, 64), (160, 1, 32), (21, 3, 128)])
+def test_any_number_of_heads_shares_a_key_head(igc_lib, kind, heads, kv, size):
+    s = Setup(igc_lib, kind, [3, 1, 2], [70, 5, 300], heads, kv, size, seed=14)
+    s.check(s.attend())
+    s.check(s.attend(window=33, sinks=2), window=33, sinks=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [2**31 - 1, 2**30 + 7, -2**31])
+def test_the_farthest_positions(igc_lib, fill):
+    """Past the cache: zeros, told.  Before it: padding."""
+    s = Setup(igc_lib, "bf16", [3, 2], [40, 9], 8, 1, 64, seed=15)
+    want, codes = s.attend(), s.cache.key_codes.clone()
+    s.fills[0] = fill
+    out = s.attend(out=torch.full_like(s.q, 5.0))
+    s.cache.write(s.k, s.v, s.fills, starts=s.starts, slots=s.slots)
+    k, v = s.cache.read(s.fills, 5, torch.float32, starts=s.starts, slots=s.slots)
+    if fill > 0:
+        with pytest.raises(igc_lib.IgcError):
+            s.cache.status()
+    s.cache.status()
+    assert out[:3].abs().max() == 0 and k[:3].abs().max() == 0 and v[:3].abs().max() == 0
+    assert torch.equal(out[3:], want[3:])
+    assert torch.equal(s.cache.key_codes[s.slot_list[0]], codes[s.slot_list[0]])
+
+
+@pytest.mark.gpu
+def test_two_streams_and_two_graphs_at_once(igc_lib):
+    """Calls on one cache from two streams, eager and captured, with scratch of
+    their own each: 4-row blocks cut between blocks, and a prompt."""
+    a = Setup(igc_lib, "bf16", [4] * 6, [900, 17, 350, 2000, 64, 1200], 8, 1, 256, seed=16)
+    q2, rows2 = a.q[:10].contiguous(), torch.tensor([0, 10], dtype=torch.int32, device="cuda")
+    f2, s2 = torch.tensor([1500], dtype=torch.int32, device="cuda"), a.slots[3:4].contiguous()
+    one = lambda: a.attend()  # noqa: E731
+    two = lambda: a.cache.attend(q2, f2, starts=rows2, slots=s2, scale=0.0625)  # noqa: E731
+    want = one(), two()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, call in zip(streams, (one, two)):
+            with torch.cuda.stream(st):
+                got.append(call())
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graphs, outs = [], []
+    for st, call in zip(streams, (one, two)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(call())
+        graphs.append(g)
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.gpu
+def test_results_in_an_array_of_other_strides(igc_lib):
+    s = Setup(igc_lib, "bf16", [5, 40], [100, 30], 8, 2, 128, seed=17)
+    want = s.attend()
+    by_head = torch.zeros(8, 45, 128, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    wide = torch.zeros(45, 8, 131, dtype=torch.bfloat16, device="cuda")[:, :, 1:129]
+    for out in (by_head, wide):
+        assert torch.equal(s.attend(out=out), want)
+    with pytest.raises(igc_lib.IgcError) as e:
+        s.attend(out=torch.zeros(45, 1, 128, dtype=torch.bfloat16, device="cuda").expand(45, 8, 128))
+    assert e.value.code == igc_lib.FAIL_ARGUMENT

@@ -105,3 +105,19 @@ def test_packed_session_refuses_bad_arguments(igc_lib):
     assert lib.igc_session_open_packed(None, 0, ctypes.byref(out)) == igc_lib.FAIL_ARGUMENT
     assert lib.igc_session_open_packed(None, -1, ctypes.byref(out)) == igc_lib.FAIL_ARGUMENT
     assert lib.igc_session_open_packed(None, 0, None) == igc_lib.FAIL_ARGUMENT
+
+
+def test_arrays_that_are_written_have_places_of_their_own(igc_lib):
+    lib = igc_lib._lib()
+    p, r, good = _pack(igc_lib), _rows(igc_lib), _data(igc_lib)
+    for kw in (dict(row_stride=0), dict(head_stride=0), dict(row_stride=good.head_stride), dict(head_stride=16)):
+        bad = _data(igc_lib, **kw)
+        assert lib.igc_pack_read(p, r, bad, good, None) == igc_lib.FAIL_ARGUMENT
+        assert lib.igc_pack_read(p, r, good, bad, None) == igc_lib.FAIL_ARGUMENT
+        assert lib.igc_pack_attend(p, r, 8, good, bad, 0, 0, 1.0, None, 0, None) == igc_lib.FAIL_ARGUMENT
+
+
+def test_places_are_counted_in_ints(igc_lib):
+    lib, r, d = igc_lib._lib(), _rows(igc_lib), _data(igc_lib)
+    p = _pack(igc_lib, slot_count=64, position_count=(1 << 24) + 64)
+    assert lib.igc_pack_write(p, r, d, d, None) == igc_lib.FAIL_ARGUMENT
