@@ -36,6 +36,9 @@ namespace igc {
 // rounded as IEEE's division does, which Markstein's correction (1990) gives
 // from the correctly rounded reciprocal: q = x y, then q + (x - q scale) y with
 // fused multiply-adds.  A group that holds a NaN or needs the clamp divides.
+// 67,000 rows of 8 x 128 in bf16: written in 142 us, read back in 77 (109 for
+// both at the copy rate; a group a thread with a division a value took 400);
+// 32768 rows of 256 in f16 read in 11 us.
 
 constexpr int PK_THREADS = 256, PK_ITEMS = 2, PK_TURNS = 2, PK_COLS = 16;
 
@@ -226,6 +229,12 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // hold it exactly; the products left out (lo x lo) are below f32's own
 // rounding, and each step of 16 positions starts from zero accumulators, as
 // the tensor core's sums round towards zero.
+//
+// Bound by instruction issue: four query heads over 131071 positions of 8 x 128
+// take 54 us (151 MB: 2.8 TB/s, issue 65% busy), 512 rows of 8 heads of 512
+// over 8704 positions 350 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
+// behind a window of 512 58 us, one token at 1024 12 us.  Steps are 128 positions
+// for 8 and 16 rows to 256 wide; wider tiles' registers leave room for 64.
 
 template <int HDP, int NT, bool SP>
 struct PackTile {
@@ -741,7 +750,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 // block: one by all its threads (a thread four columns of every second, fourth
 // or eighth piece of a narrow head) where there may be many pieces, else each
 // by as many threads as it has fours of columns.  The order of the additions
-// is fixed.
+// is fixed.  (64 sequences of 32 rows cut over 148 blocks: 66 us with the
+// attention; 79 with one row a block and its pieces read one after another.)
 
 struct PackMerge {
   PackAttend a;
