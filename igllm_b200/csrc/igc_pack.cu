@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // Bound by instruction issue: four query heads over 131071 positions of 8 x 128
 // take 54 us (151 MB: 2.8 TB/s, issue 65% busy), 512 rows of 8 heads of 512
 // over 8704 positions 350 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
-// behind a window of 512 58 us, one token at 1024 12 us.  Steps are 128 positions
+// behind a window of 512 58 us, one token at 1024 9 us.  Steps are 128 positions
 // for 8 and 16 rows to 256 wide; wider tiles' registers leave room for 64.
 
 template <int HDP, int NT, bool SP>
@@ -266,6 +266,8 @@ struct PackTile {
   static constexpr int PF = TP / 16 * NT * 256;          // bytes of one part's weight fragments
   static constexpr int OFF_P = OFF_SUM + 4 * RB * 4;
   static constexpr int SMEM = 1024 + OFF_P + PF * PARTS;
+  static_assert(RING >= RB * (HDP + 2) * 4, "a cluster's partial sums lie in the ring");
+  static constexpr bool CLUSTERS = NT <= 2;              // may share a unit as a cluster (the wider forms have no registers for it)
   // blocks an SM that registers are kept for
   static constexpr int PER_SM = NT == 1 ? (HDP <= 128 ? 4 : 3) : NT <= 4 && HDP <= 256 ? 3 : 2;
 };
@@ -282,10 +284,59 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
   return y;
 }
+
+// A cluster's partial sums, each block's in its own shared memory as pieces lie
+// in global, joined; a block takes its share of the fours of columns.
+template <int RB>
+__device__ __forceinline__ void join_cluster(const PackAttend &a, const PackWalk &w, const float *mine, int cluster) {
+  cluster_sync();
+  const int size = a.c.size, fours = size / 4, all = min(RB, w.q.n * a.group) * fours;
+  const int rank = blockIdx.x % cluster;
+  const bool wide = wide_rows(a.out);
+  for (int i = rank * 128 + threadIdx.x; i < all; i += cluster * 128) {
+    const int r = i / fours, col = 4 * (i - r * fours);
+    float m = -INFINITY, l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = 0; j0 < cluster; j0 += 4) {
+      float pm[4], pl[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        pl[k] = 0.0f;
+        pm[k] = -INFINITY;
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j0 + k < cluster) {
+          pm[k] = cluster_ld(mine + RB * size + r, j0 + k);
+          pl[k] = cluster_ld(mine + RB * size + RB + r, j0 + k);
+          v[k] = cluster_ld4(mine + r * size + col, j0 + k);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float mx = fmaxf(m, pm[k]), base = mx == -INFINITY ? 0.0f : mx;
+        const float back = exp2_fast(m - base), f = exp2_fast(pm[k] - base);
+        m = mx;
+        l = l * back + pl[k] * f;
+        x[0] = fmaf(v[k].x, f, x[0] * back);
+        x[1] = fmaf(v[k].y, f, x[1] * back);
+        x[2] = fmaf(v[k].z, f, x[2] * back);
+        x[3] = fmaf(v[k].w, f, x[3] * back);
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
+    const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+    const int token = a.by_group.of(r);
+    store4(a.out.data, a.out.type,
+           (size_t)(w.q.first + token) * a.out.row_stride +
+               (size_t)(w.h * a.group + r - token * a.group) * a.out.head_stride + col,
+           wide, y);
+  }
+  cluster_sync();  // no block ends before the others have read its sums
+}
+
 template <int HDP, int NT, bool SP, bool FULL>
 __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     pack_attend_kernel(const __grid_constant__ PackAttend a, const __grid_constant__ CUtensorMap tmk,
-                       const __grid_constant__ CUtensorMap tmv, int tall) {
+                       const __grid_constant__ CUtensorMap tmv, int tall, int cluster) {
   using L = PackTile<HDP, NT, SP>;
   constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, MP = L::MP, TP = L::TP,
                 PITCH = L::PITCH;
@@ -313,10 +364,25 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
   }
 
   PackWalk w;
-  int share;
-  const bool any = walk_start<RB, TP, L::OVER>(a, tall, w, &share);
+  int share = 0;
+  bool any;
+  if (!L::CLUSTERS) cluster = 0;
+  if (cluster > 0) {  // a unit a cluster: the blocks take runs of its tiles
+    const int unit = blockIdx.x / cluster, rank = blockIdx.x - unit * cluster;
+    w.s = unit / a.c.heads;
+    w.h = unit - w.s * a.c.heads;
+    w.b = 0;
+    w.q = seq_at(a.c, a.r, w.s);
+    w.sp = block_span(a, w.q, 0, RB, TP);
+    w.ka = w.sp.count() * rank / cluster;
+    w.kb = w.sp.count() * (rank + 1) / cluster;
+    w.whole = cluster == 1;
+    any = w.q.n > 0;
+  } else {
+    any = walk_start<RB, TP, L::OVER>(a, tall, w, &share);
+  }
   pdl_release();
-  if (tid == 0) leave_cut(a, w, any);
+  if (cluster == 0 && tid == 0) leave_cut(a, w, any);
   if (!any) return;
   int step0 = 0;  // steps this block has taken: the ring's place
   bool gave_up = false;
@@ -710,7 +776,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     }
     if (wp == 0) {
       const bool wide = wide_rows(a.out);
-      float *pw = piece_at(a, gridDim.x, RB, 2 * (size_t)blockIdx.x + (ka == 0 ? 1 : 0));
+      float *pw = cluster > 0 ? reinterpret_cast<float *>(sm)
+                              : piece_at(a, gridDim.x, RB, 2 * (size_t)blockIdx.x + (ka == 0 ? 1 : 0));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -739,6 +806,10 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
         }
     }
 
+    if (cluster > 0) {
+      if (cluster > 1) join_cluster<RB>(a, w, reinterpret_cast<const float *>(sm), cluster);
+      break;
+    }
     if (!walk_next<RB, TP, L::OVER>(a, w, share)) break;
   }
   if (gave_up) pack_trouble(a.c);
@@ -874,6 +945,7 @@ cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
   if (dev < PACK_DEVICES && (*per_sm = known[dev].load()) > 0) return cudaSuccess;
   auto kern = pack_attend_kernel<HDP, NT, SP, FULL>;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kern, 128, L::SMEM);
   if (e == cudaSuccess && *per_sm < 1) e = cudaErrorInvalidConfiguration;
   if (e == cudaSuccess && dev < PACK_DEVICES) known[dev].store(*per_sm);
@@ -883,8 +955,8 @@ cudaError_t pack_form_ready(PackPlan *plan, int *per_sm) {
 template <int HDP, int NT, bool SP, bool FULL>
 cudaError_t pack_form_launch(const PackAttend &a, const PackPlan &p, const CUtensorMap &tmk, const CUtensorMap &tmv,
                              cudaStream_t st) {
-  return pack_launch(pack_attend_kernel<HDP, NT, SP, FULL>, dim3(p.grid), 128, PackTile<HDP, NT, SP>::SMEM, st, false, a,
-                     tmk, tmv, p.tall);
+  return pack_launch(pack_attend_kernel<HDP, NT, SP, FULL>, dim3(p.grid), 128, PackTile<HDP, NT, SP>::SMEM, st, false, p.cluster,
+                     a, tmk, tmv, p.tall, p.cluster);
 }
 
 // Calls F for the form a plan names.
@@ -972,7 +1044,7 @@ static cudaError_t launch_rows(const PackView *c, const PackRows *r, const PackD
     return ((size_t)d.data & 15) == 0 && d.row_stride % per == 0 && d.head_stride % per == 0;
   };
   const bool wide = lies(*k) && lies(*v);
-  auto run = [&](auto kern) { return pack_launch(kern, grid, PK_THREADS, 0, st, false, io); };
+  auto run = [&](auto kern) { return pack_launch(kern, grid, PK_THREADS, 0, st, false, 0, io); };
   switch (k->type * 2 + (wide ? 1 : 0)) {
     case 2: return run(pack_rows_kernel<WRITE, 1, false>);
     case 3: return run(pack_rows_kernel<WRITE, 1, true>);
@@ -1018,6 +1090,21 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   const long tiles = ((reach < positions ? reach : positions) + p->tile - 1) / p->tile;
   const double list = ((double)rows * group / rb + count) * kv_heads * (tiles + p->over);
   if (list >= 2147483648.0) return cudaErrorInvalidValue;
+  // Few units of few tiles: a cluster of blocks a unit, joined there, one
+  // launch and no scratch (one token at 1024 positions 11.6 -> 9.1 us, 64 tokens
+  // behind a window of 512 17 -> 12.4).  Where blocks would take more than four
+  // tiles each or not all run at once, the list keeps more of the device busy.
+  if (!p->tc && p->rows8 <= 2 && blocks == 1) {
+    const long units = (long)count * kv_heads, wave = (long)sms * per_sm;
+    int cluster = 1;
+    while (cluster < 16 && cluster < tiles) cluster *= 2;
+    while (cluster > 1 && units * cluster > wave) cluster /= 2;
+    if (tiles <= 4 * cluster && units * cluster <= wave) {
+      p->cluster = cluster;
+      p->grid = (int)units * cluster;
+      return cudaSuccess;
+    }
+  }
   p->grid = sms * per_sm;
   if (list < p->grid) p->grid = (int)list < 1 ? 1 : (int)list;
   p->tall = blocks > 8;
@@ -1060,9 +1147,9 @@ cudaError_t igc_launch_pack_attend(const PackAttend *a, const PackPlan *p, cudaS
   if (e != cudaSuccess) return e;
   *launches = 1;
   e = p->tc ? igc_launch_pack_tc(a, p, &tmk, &tmv, st) : pack_run(*p, *a, tmk, tmv, st);
-  if (e != cudaSuccess || p->grid == 1) return e;
+  if (e != cudaSuccess || p->grid == 1 || p->cluster > 0) return e;
   *launches = 2;
   const int rb = 8 * p->rows8, some = p->tc && PM_THREADS / (a->c.size / 4) >= 2 ? 2 : 1;
   const PackMerge g = {*a, rb, p->grid, some};
-  return pack_launch(pack_merge_kernel, dim3((unsigned)p->grid - 1, rb / some), PM_THREADS, 0, st, true, g);
+  return pack_launch(pack_merge_kernel, dim3((unsigned)p->grid - 1, rb / some), PM_THREADS, 0, st, true, 0, g);
 }

@@ -173,6 +173,26 @@ __device__ __forceinline__ void pk_load(void *dst, const CUtensorMap *map, int x
       : "memory");
 }
 
+// What lies at `p` in the shared memory of cluster block `rank`.
+__device__ __forceinline__ uint32_t cluster_at(const float *p, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float cluster_ld(const float *p, int rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(x) : "r"(cluster_at(p, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 cluster_ld4(const float *p, int rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(cluster_at(p, rank))
+               : "memory");
+  return x;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -393,20 +413,26 @@ __device__ __forceinline__ float *piece_at(const PackAttend &a, int grid, int rb
   return a.work + (size_t)grid * (sizeof(PackCut) / 4) + i * ((size_t)rb * (a.c.size + 2));
 }
 
+// `overlap`: may start before the kernel ahead ends; `cluster`: blocks of one (0: none).
 template <typename... P, typename... Q>
 cudaError_t pack_launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool overlap,
-                        Q... args) {
+                        int cluster, Q... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
   if (overlap) {
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = 1;
+    at[cfg.numAttrs++].val.clusterDim.z = 1;
   }
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }

@@ -72,6 +72,7 @@ struct PackPlan {
   int over;      // steps a unit costs beside its own
   int pitch;     // code bytes of a row of a TMA box
   int tall;      // some sequence has many blocks of rows
+  int cluster;   // blocks of a cluster that share a unit, 0: the list of tiles instead
   int grid;
   size_t work_floats;
 };

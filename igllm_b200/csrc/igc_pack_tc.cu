@@ -34,8 +34,8 @@
 // room for.  3 prompts to 4096 of 8 x 256: 122 us, 640 TFLOP/s; 8192 rows behind
 // a window of 512: 100 us; 64 x 4 rows at 8192: 66 us.  The mma.sync form took
 // 506, 355 and 104.  A unit's ends (queries in, results out) cost about 8 steps,
-// which OVER tells the sharing (4, 7, 8 and 10 measured: 64 x 4 in 86, 81, 80 and
-// 83 us, prompts in 164, 127, 126 and 131, before the joining was sped up).
+// which OVER tells the sharing (4, 7 and 10 measured: 64 x 4 in 86, 81 and 83 us,
+// prompts in 164, 127 and 131, before the joining was sped up).
 #include <atomic>
 
 #include "igc_pack.cuh"
@@ -710,7 +710,7 @@ static cudaError_t tc_ready(PackPlan *plan) {
 template <int HDP>
 static cudaError_t tc_run(const PackAttend &a, const PackPlan &p, const CUtensorMap &tmk, const CUtensorMap &tmv,
                           cudaStream_t st) {
-  return pack_launch(pack_attend_tc_kernel<HDP>, dim3(p.grid), TC_THREADS, PackTc<HDP>::SMEM, st, false, a, tmk, tmv,
+  return pack_launch(pack_attend_tc_kernel<HDP>, dim3(p.grid), TC_THREADS, PackTc<HDP>::SMEM, st, false, 0, a, tmk, tmv,
                      p.tall);
 }
 

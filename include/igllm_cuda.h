@@ -393,7 +393,7 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * and the softmax are f32; queries are read as f16 after an exact power of two
  * a row, and for F32 rows every product keeps both halves of a hi/lo split, so
  * that results hold to f32.  `work` is device scratch of at least the bytes
- * igc_pack_attend_room gives for the same arguments (a multiple of 16 bytes
+ * igc_pack_attend_room gives for the same arguments (often none; a multiple of 16 bytes
  * aligned); calls that may run at once need scratch of their own.
  *
  * Each call makes pack->device current and restores the caller's device; work
