@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // Bound by instruction issue: four query heads over 131071 positions of 8 x 128
 // take 54 us (151 MB: 2.8 TB/s, issue 65% busy), 512 rows of 8 heads of 512
 // over 8704 positions 350 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
-// behind a window of 512 58 us, one token at 1024 9 us.  Steps are 128 positions
+// behind a window of 512 44 us, one token at 1024 9 us.  Steps are 128 positions
 // for 8 and 16 rows to 256 wide; wider tiles' registers leave room for 64.
 
 template <int HDP, int NT, bool SP>
@@ -290,7 +290,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 template <int RB>
 __device__ __forceinline__ void join_cluster(const PackAttend &a, const PackWalk &w, const float *mine, int cluster) {
   cluster_sync();
-  const int size = a.c.size, fours = size / 4, all = min(RB, w.q.n * a.group) * fours;
+  const int size = a.c.size, fours = size / 4, all = min(RB, w.q.n * a.group - w.b * RB) * fours;
   const int rank = blockIdx.x % cluster;
   const bool wide = wide_rows(a.out);
   for (int i = rank * 128 + threadIdx.x; i < all; i += cluster * 128) {
@@ -324,10 +324,10 @@ __device__ __forceinline__ void join_cluster(const PackAttend &a, const PackWalk
     }
     const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
     const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
-    const int token = a.by_group.of(r);
+    const int rr = w.b * RB + r, token = a.by_group.of(rr);
     store4(a.out.data, a.out.type,
            (size_t)(w.q.first + token) * a.out.row_stride +
-               (size_t)(w.h * a.group + r - token * a.group) * a.out.head_stride + col,
+               (size_t)(w.h * a.group + rr - token * a.group) * a.out.head_stride + col,
            wide, y);
   }
   cluster_sync();  // no block ends before the others have read its sums
@@ -369,15 +369,17 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
   if (!L::CLUSTERS) cluster = 0;
   if (cluster > 0) {  // a unit a cluster: the blocks take runs of its tiles
     const int unit = blockIdx.x / cluster, rank = blockIdx.x - unit * cluster;
-    w.s = unit / a.c.heads;
-    w.h = unit - w.s * a.c.heads;
-    w.b = 0;
+    const int block = unit / a.c.heads;
+    w.h = unit - block * a.c.heads;
+    w.s = block / tall;
+    w.b = block - w.s * tall;
     w.q = seq_at(a.c, a.r, w.s);
-    w.sp = block_span(a, w.q, 0, RB, TP);
+    any = w.b < blocks_of(a, w.q, RB);
+    if (any) w.sp = block_span(a, w.q, w.b, RB, TP);
+    else w.sp = {0, 0, 0, 0, 0};
     w.ka = w.sp.count() * rank / cluster;
     w.kb = w.sp.count() * (rank + 1) / cluster;
     w.whole = cluster == 1;
-    any = w.q.n > 0;
   } else {
     any = walk_start<RB, TP, L::OVER>(a, tall, w, &share);
   }
@@ -1065,48 +1067,64 @@ cudaError_t igc_launch_pack_read(const PackView *c, const PackRows *r, const Pac
   return launch_rows<false>(c, r, k, v, st);
 }
 
+// The most tiles a unit of blocks of `rb` rows has: the rows' reach, wherever it
+// starts in a tile.
+static long most_tiles(const PackPlan *p, int rb, int positions, int group, int window, int sinks) {
+  const long reach = window > 0 ? (long)window + rb / group + 1 + sinks + 3 * p->tile : positions;
+  return ((reach < positions ? reach : positions) + p->tile - 1) / p->tile;
+}
+
 cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int kv_heads, int group, int size,
                           int type, int window, int sinks, PackPlan *p) {
   memset(p, 0, sizeof(*p));
   p->wide = size <= 64 ? 64 : size <= 128 ? 128 : size <= 256 ? 256 : 512;
   p->split2 = type == 1 ? 1 : 0;
+  p->full = size == p->wide;
   const long need = (long)rows_most * group;
+  int sms = 0, per_sm = 0;
+  cudaError_t e = pack_sms(&sms);
+  // Few units of few tiles: a cluster of blocks a unit, joined there, one
+  // launch and no scratch (one token at 1024 positions 11.6 -> 9.1 us, 64 tokens
+  // behind a window of 512 17 -> 12.4; 4 lanes of 8 heads of 256 at 1024, in 32
+  // bits 20.6 -> 8.9, in 16, against the tcgen05 form, 17.8 -> 8.7).  That holds to
+  // eight tiles a block (100 tokens at 1000: 21.8 us, the list 27.9; 4 lanes at
+  // 16000 28 and 41), but to four where the largest clusters of single blocks of
+  // rows leave most of the device idle (one token at 8100: 17 us and 20, at 16000
+  // 28 and 23).  Sixteen rows a block where eight would not do, of full heads only.
+  for (int rows8 = 1; rows8 <= (p->full && need > 8 ? 2 : 1) && e == cudaSuccess; ++rows8) {
+    p->rows8 = rows8;
+    e = pack_form(p, &per_sm);
+    const long blocks = (need + 8 * rows8 - 1) / (8 * rows8), units = (long)count * kv_heads * blocks;
+    const long wave = (long)sms * per_sm, tiles = most_tiles(p, 8 * rows8, positions, group, window, sinks);
+    int cluster = 1;
+    while (cluster < 16 && cluster < tiles) cluster *= 2;
+    while (cluster > 1 && units * cluster > wave) cluster /= 2;
+    if (e == cudaSuccess && units * cluster <= wave && tiles <= (cluster == 16 && blocks == 1 ? 4 : 8) * cluster) {
+      p->cluster = cluster;
+      p->tall = (int)blocks;
+      p->grid = (int)units * cluster;
+      return cudaSuccess;
+    }
+  }
+  if (e != cudaSuccess) return e;
   int most8 = p->split2 ? 4 : 2;  // what registers hold, and past 16 rows the tcgen05 form takes over
   if (p->wide == 512) most8 = p->split2 ? 2 : 4;
-  p->full = size == p->wide;
   p->rows8 = need <= 8 ? 1 : need <= 16 && p->full ? 2 : most8;  // fewer forms where a group's tile is part empty
   if (!p->split2 && p->wide <= 256 && need > 16) {
     p->tc = 1;
     p->rows8 = 16;
   }
   const int rb = 8 * p->rows8;
-  int sms = 0, per_sm = 0;
-  cudaError_t e = pack_sms(&sms);
-  if (e == cudaSuccess) e = pack_form(p, &per_sm);
+  e = pack_form(p, &per_sm);
   if (e != cudaSuccess) return e;
-  const long blocks = (need + rb - 1) / rb;
-  // no more blocks than the most tiles there can be: the rows' reach, wherever it starts in a tile
-  const long reach = window > 0 ? (long)window + rb / group + 1 + sinks + 3 * p->tile : positions;
-  const long tiles = ((reach < positions ? reach : positions) + p->tile - 1) / p->tile;
+  const long blocks = (need + rb - 1) / rb, tiles = most_tiles(p, rb, positions, group, window, sinks);
   const double list = ((double)rows * group / rb + count) * kv_heads * (tiles + p->over);
   if (list >= 2147483648.0) return cudaErrorInvalidValue;
-  // Few units of few tiles: a cluster of blocks a unit, joined there, one
-  // launch and no scratch (one token at 1024 positions 11.6 -> 9.1 us, 64 tokens
-  // behind a window of 512 17 -> 12.4).  Where blocks would take more than four
-  // tiles each or not all run at once, the list keeps more of the device busy.
-  if (!p->tc && p->rows8 <= 2 && blocks == 1) {
-    const long units = (long)count * kv_heads, wave = (long)sms * per_sm;
-    int cluster = 1;
-    while (cluster < 16 && cluster < tiles) cluster *= 2;
-    while (cluster > 1 && units * cluster > wave) cluster /= 2;
-    if (tiles <= 4 * cluster && units * cluster <= wave) {
-      p->cluster = cluster;
-      p->grid = (int)units * cluster;
-      return cudaSuccess;
-    }
-  }
+  // blocks of at least 7 steps, were all units as long as they can be: shorter runs
+  // leave more pieces to join than they save (one token at 32000: 49 us by single
+  // steps, 29 by 4, 28 by 7; 100000: 60, 60, 53)
   p->grid = sms * per_sm;
-  if (list < p->grid) p->grid = (int)list < 1 ? 1 : (int)list;
+  if (list / 7 < p->grid) p->grid = list < 7 ? 1 : (int)(list / 7);
   p->tall = blocks > 8;
   p->work_floats = p->grid > 1 ? (size_t)p->grid * (8 + 2 * (size_t)rb * (size + 2)) : 8;
   return cudaSuccess;

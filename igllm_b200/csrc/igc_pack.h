@@ -71,7 +71,7 @@ struct PackPlan {
   int tile;      // positions a step
   int over;      // steps a unit costs beside its own
   int pitch;     // code bytes of a row of a TMA box
-  int tall;      // some sequence has many blocks of rows
+  int tall;      // some sequence has many blocks of rows; with clusters, the most of any
   int cluster;   // blocks of a cluster that share a unit, 0: the list of tiles instead
   int grid;
   size_t work_floats;

@@ -547,3 +547,25 @@ def test_results_in_an_array_of_other_strides(igc_lib):
     with pytest.raises(igc_lib.IgcError) as e:
         s.attend(out=torch.zeros(45, 1, 128, dtype=torch.bfloat16, device="cuda").expand(45, 8, 128))
     assert e.value.code == igc_lib.FAIL_ARGUMENT
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,kv,size", [("f32", 4, 2, 64), ("bf16", 8, 2, 128), ("f16", 3, 3, 512),
+                                                ("f32", 8, 2, 256), ("bf16", 10, 2, 96)])
+def test_many_ragged_sequences(igc_lib, kind, heads, kv, size):
+    """More units than run at once: one list of tiles, shared out in runs that
+    begin and end anywhere; empty sequences, padding, and rows of 0 to 2."""
+    g = np.random.default_rng(18)
+    rows = [int(x) for x in g.integers(0, 3, 330)]
+    fill = [int(x) for x in np.where(g.random(330) < 0.1, -1, g.integers(0, 400, 330))]
+    s = Setup(igc_lib, kind, rows, fill, heads, kv, size, seed=19)
+    s.check(s.attend(rows_most=2))
+    s.check(s.attend(rows_most=2, window=70, sinks=5), window=70, sinks=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,kv,size", [("f32", 8, 1, 256), ("bf16", 8, 2, 128), ("f16", 4, 1, 512)])
+@pytest.mark.parametrize("rows,depth", [(1, 4200), (5, 1500), (20, 700), (3, 16200)])
+def test_few_units_in_clusters(igc_lib, kind, heads, kv, size, rows, depth):
+    s = Setup(igc_lib, kind, [rows, max(1, rows - 2)], [depth, depth // 3], heads, kv, size, seed=20)
+    s.check(s.attend(rows_most=rows))
