@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // the tensor core's sums round towards zero.
 //
 // Bound by instruction issue: four query heads over 131071 positions of 8 x 128
-// take 54 us (151 MB: 2.8 TB/s, issue 65% busy), 512 rows of 8 heads of 512
-// over 8704 positions 350 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
+// take 56 us (151 MB: 2.7 TB/s, issue 65% busy), 512 rows of 8 heads of 512
+// over 8704 positions 353 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
 // behind a window of 512 44 us, one token at 1024 9 us.  Steps are 128 positions
 // for 8 and 16 rows to 256 wide; wider tiles' registers leave room for 64.
 
