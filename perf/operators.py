@@ -130,9 +130,7 @@ def work(case):
 def _pack(x):
     """Rows of 32-bit values to (codes two a byte, f16 scales)."""
     g = x.unflatten(-1, (-1, GROUP))
-    big = g.abs().amax(-1)
-    # a tensor of sevens: by a number, torch multiplies by its reciprocal, which is another rounding
-    scale = torch.clamp(big / torch.full_like(big, 7.0), max=SCALE_MOST).to(torch.float16)
+    scale = torch.clamp(g.abs().amax(-1) / 7.0, max=SCALE_MOST).to(torch.float16)
     step = scale.to(torch.float32).unsqueeze(-1)
     code = torch.clamp(torch.round(g / torch.where(step > 0, step, 1.0)), -8, 7)
     code = (torch.where(step > 0, code, 0.0) + 8).to(torch.uint8).flatten(-2)
