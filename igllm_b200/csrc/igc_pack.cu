@@ -218,9 +218,14 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 //           maximum is merged through shared memory once a tile.
 //   values  warp w takes 64 of the head's columns (or, of a narrow head, a
 //           share of the positions).  Codes of two positions are zipped by a
-//           byte permute, used as they lie.  For 16-bit rows the group's
-//           scale goes into the weight, f16(f16(w) 8 scale), two roundings of
-//           2^-11 at most, and codes enter exactly.
+//           byte permute, used as they lie.  For 16-bit rows a weight and a
+//           value are each rounded to f16 once: the value f16((n - 8) scale),
+//           a whole number of 2^-24 however small the scale (2^-11 of it at
+//           most), and the weight 2^15 times itself (2^-11 of it at most down
+//           to 2^-29 of the row's largest, below that 2^-40 of the largest).
+//           Folded into the weight instead, small scales took the product
+//           below f16's range, and first positions of much weight and small
+//           values took the rest of the row's result with them.
 //
 // A query row is scaled by the power of two that puts its largest magnitude
 // in [2^13, 2^14) and kept as f16, exact for bf16 and f16 rows but for
@@ -338,6 +343,7 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     pack_attend_kernel(const __grid_constant__ PackAttend a, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, int tall, int cluster) {
   using L = PackTile<HDP, NT, SP>;
+  constexpr float WEIGHT = SP ? 4096.0f : 32768.0f;  // what weights, and with them sums and results, are kept times
   constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, MP = L::MP, TP = L::TP,
                 PITCH = L::PITCH;
   extern __shared__ __align__(1024) uint8_t sm_raw[];
@@ -609,9 +615,7 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
         for (int mp = 0; mp < MP; ++mp) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // f32 rows: 2^12 the weight, so that its halves reach 2^-37 of the largest
-            const float x = exp2_fast(sc[mp][nt][e] - base[e & 1]);
-            sc[mp][nt][e] = SP ? x * 4096.0f : x;
+            sc[mp][nt][e] = exp2_fast(sc[mp][nt][e] - base[e & 1]) * WEIGHT;
             sum[e & 1] += sc[mp][nt][e];
           }
           // the weights turned to the second product's fragment: positions along its depth
@@ -694,20 +698,11 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                   for (int e = 0; e < 2; ++e) {
-                    const uint32_t c = v[2 * u + e];
-                    if (SP) {
-                      const uint32_t hi = mul2(c, step[i]);
-                      av[u][2 * i + e] = hi;
-                      al[u][2 * i + e] = rest2(c, step[i], hi);
-                    } else {
-                      av[u][2 * i + e] = c;
-                    }
+                    const uint32_t c = v[2 * u + e], hi = mul2(c, step[i]);
+                    av[u][2 * i + e] = hi;
+                    if (SP) al[u][2 * i + e] = rest2(c, step[i], hi);
                   }
               }
-            if (!SP) {
-              step[0] = mul2(step[0], 0x48004800u);  // 8: weights of small scales stay above f16's smallest
-              step[1] = mul2(step[1], 0x48004800u);
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               if (SP) {
@@ -721,9 +716,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
                   for (int e = 0; e < 4; ++e) o[nt][nb * 4 + gi * 2 + u][e] += acc[e];
                 }
               } else {
-                const uint32_t b0 = mul2(pb[0][nt].x, step[0]), b1 = mul2(pb[0][nt].y, step[1]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) mma_add(o[nt][nb * 4 + gi * 2 + u], av[u], b0, b1);
+                for (int u = 0; u < 2; ++u) mma_add(o[nt][nb * 4 + gi * 2 + u], av[u], pb[0][nt].x, pb[0][nt].y);
               }
             }
           }
@@ -731,14 +725,6 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
       }
     }
     step0 += kb - ka;
-    if (!SP) {  // undo the 8 the weights carried
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < NB * 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][j][e] *= 0.125f;
-    }
 
     // ---- the rows' sums, and of a narrow head the warps' shares, joined
 #pragma unroll
