@@ -230,9 +230,10 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // A query row is scaled by the power of two that puts its largest magnitude
 // in [2^13, 2^14) and kept as f16, exact for bf16 and f16 rows but for
 // magnitudes 2^38 below the largest.  For f32 rows (SP) queries and weights
-// are each kept as f16 hi and lo parts and (n - 8) scale as hi and lo, which
-// hold it exactly; the products left out (lo x lo) are below f32's own
-// rounding, and each step of 16 positions starts from zero accumulators, as
+// are each kept as f16 hi and lo parts, a weight's lo 2^11 times itself (its
+// hi 2^15 times, so that both hold to 2^-51 of the row's largest), and
+// (n - 8) scale as hi and lo, which hold it exactly; the products left out
+// (lo x lo) are below f32's own rounding, and each step of 16 positions starts from zero accumulators, as
 // the tensor core's sums round towards zero.
 //
 // Bound by instruction issue: four query heads over 131071 positions of 8 x 128
@@ -343,7 +344,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
     pack_attend_kernel(const __grid_constant__ PackAttend a, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, int tall, int cluster) {
   using L = PackTile<HDP, NT, SP>;
-  constexpr float WEIGHT = SP ? 4096.0f : 32768.0f;  // what weights, and with them sums and results, are kept times
+  constexpr float WEIGHT = 32768.0f;  // what weights, and with them sums and results, are kept times
+  constexpr float LOW = 2048.0f;      // what their low halves are kept times beside it
   constexpr int RB = L::RB, C = L::C, NS = L::NS, WC = L::WC, WP = L::WP, NB = L::NB, MP = L::MP, TP = L::TP,
                 PITCH = L::PITCH;
   extern __shared__ __align__(1024) uint8_t sm_raw[];
@@ -625,8 +627,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
           if (SP) {
             const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
             const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
-            const uint32_t l0 = half2_bits(sc[mp][nt][0] - f0.x, sc[mp][nt][1] - f0.y);
-            const uint32_t l1 = half2_bits(sc[mp][nt][2] - f1.x, sc[mp][nt][3] - f1.y);
+            const uint32_t l0 = half2_bits((sc[mp][nt][0] - f0.x) * LOW, (sc[mp][nt][1] - f0.y) * LOW);
+            const uint32_t l1 = half2_bits((sc[mp][nt][2] - f1.x) * LOW, (sc[mp][nt][3] - f1.y) * LOW);
             p[L::PF / 8] = make_uint2(transpose8(l0), transpose8(l1));
           }
         }
@@ -709,8 +711,10 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                  mma_add(acc, al[u], pb[0][nt].x, pb[0][nt].y);
                   mma_add(acc, av[u], pb[L::PARTS - 1][nt].x, pb[L::PARTS - 1][nt].y);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[e] *= 1.0f / LOW;
+                  mma_add(acc, al[u], pb[0][nt].x, pb[0][nt].y);
                   mma_add(acc, av[u], pb[0][nt].x, pb[0][nt].y);
 #pragma unroll
                   for (int e = 0; e < 4; ++e) o[nt][nb * 4 + gi * 2 + u][e] += acc[e];

@@ -81,6 +81,14 @@ def test_first_positions_that_hold_the_weight(igc_lib, kind, above, window, rows
     check(s, window=window, sinks=4 if window else 0, above=above)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,depth,heads,size", FEW + MANY)
+def test_first_positions_far_above_in_32_bits(igc_lib, rows, depth, heads, size):
+    s = Setup(igc_lib, "f32", [rows], [depth], heads, 1, size, seed=size + rows)
+    stand_out(s, 20)
+    check(s, above=20)
+
+
 def stand_out(s, above):
     """Columns 0 to 31 of every query are 1, and of the keys 7 scale in the
     first four positions and 0 in the others."""
