@@ -690,6 +690,14 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
               const uint32_t w1 = *reinterpret_cast<const uint32_t *>(box + (vat[1] ^ j));
               x[i] = __byte_perm(w0, w1, zip);
             }
+            // f32 rows: scales all below 2^-7 (0x2000) go in 2^13 times, as the tensor core aligns
+            // products by their exponent fields and would cut those of subnormal values short
+            float back = 1.0f;
+            if (SP && __all_sync(0xffffffffu, ((step[0] | step[1]) & 0xe000e000u) == 0)) {
+              step[0] = mul2(step[0], 0x70007000u);
+              step[1] = mul2(step[1], 0x70007000u);
+              back = 1.0f / 8192.0f;
+            }
             // product u: columns 2u (rows 0-7) and 2u + 1 (rows 8-15) of the thread's four
             uint32_t av[2][4], al[2][4];
 #pragma unroll
@@ -717,7 +725,8 @@ __global__ void __launch_bounds__(128, PackTile<HDP, NT, SP>::PER_SM)
                   mma_add(acc, al[u], pb[0][nt].x, pb[0][nt].y);
                   mma_add(acc, av[u], pb[0][nt].x, pb[0][nt].y);
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) o[nt][nb * 4 + gi * 2 + u][e] += acc[e];
+                  for (int e = 0; e < 4; ++e)
+                    o[nt][nb * 4 + gi * 2 + u][e] = fmaf(acc[e], back, o[nt][nb * 4 + gi * 2 + u][e]);
                 }
               } else {
 #pragma unroll

@@ -61,8 +61,8 @@ MANY = [(4, 20011, 8, 256), (4, 20011, 8, 64), (40, 17001, 8, 96)]  # more than 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,depth,heads,size", FEW + MANY)
-@pytest.mark.parametrize("kind,step", [("f32", 1e-4), ("bf16", 1e-4), ("bf16", 1e-6), ("bf16", 2.0 ** -24),
-                                       ("f16", 2.0 ** -8)])
+@pytest.mark.parametrize("kind,step", [("f32", 1e-4), ("f32", 2.0 ** -24), ("bf16", 1e-4), ("bf16", 1e-6),
+                                       ("bf16", 2.0 ** -24), ("f16", 2.0 ** -8)])
 def test_values_of_any_size(igc_lib, kind, step, rows, depth, heads, size):
     s = Setup(igc_lib, kind, [rows], [depth], heads, 1, size, seed=size + rows)
     s.cache.value_scales.fill_(step)
