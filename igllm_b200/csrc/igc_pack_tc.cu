@@ -19,13 +19,17 @@
 //                    maximum, the weights back into tensor memory, the row's
 //                    sum.  The maximum in use is handed from tile to tile; it
 //                    and the results change only when a tile's maximum is more
-//                    than 2^8 over it, as weights stay below f16's range until
-//                    then.
+//                    than 2^8 over it.  Weights are kept 2^7 times, which then
+//                    still fits f16.  (Following by 2^4, 2^2 or at once, with
+//                    weights 2^11 to 2^15 times, takes prompts 128 us to 135,
+//                    171, 180 and the windowed prompt 102 to 125.)
 //
 // Columns of a group of eight keep the order their nibbles come out in,
 // 0 4 1 5 2 6 3 7, in the queries and, undone at the end, in the results.
 // A bf16 query row is scaled by an exact power of two into f16's range; keys,
-// values and weights are each rounded to f16 once (2^-11 at most).
+// values and weights are each rounded to f16 once: 2^-11 of a key or value at
+// most, which are whole numbers of 2^-24 whatever their scale, and 2^-11 of a
+// weight down to 2^-21 of the row's largest, below that 2^-32 of the largest.
 //
 // Bound by the products: a step of a 256-wide head is 16 score products of 53
 // cycles (64 positions wide: 61% of the pipe's rate) and 4 value products of 129
@@ -46,6 +50,8 @@ template <int HDP>
 struct PackTc {
   static constexpr int RB = 128, TP = 64, C = HDP / 32;
   static constexpr int OVER = 8;                        // steps a unit costs beside its own
+  static constexpr int LAG = 8;                         // powers of two a maximum in use may be passed by
+  static constexpr int KEEP = 15 - LAG;                 // power of two that weights, sums and results are kept times
   static constexpr int BLOCKS = HDP / 64;               // 64-column blocks of an operand
   static constexpr int SIDE = BLOCKS * 64 * 128;        // one key or value operand buffer
   static constexpr int T_S = HDP;                       // tensor-memory columns: results, then four tiles of scores
@@ -136,6 +142,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t mulf2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 __device__ __forceinline__ float first2(uint64_t a) { return __uint_as_float((uint32_t)a); }
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             wait(&mtold[(T - 1) & 1], (T - 1) >> 1);
             now = shared_m[(T - 1) & 1][r];
           }
-          const bool grown = top > now && (now == -INFINITY || (top - now) * f > 8.0f);
+          const bool grown = top > now && (now == -INFINITY || (top - now) * f > (float)L::LAG);
           const float before = now;
           if (grown) now = top;
           shared_m[T & 1][r] = now;
@@ -566,15 +577,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               }
             }
             const float base = now == -INFINITY ? 0.0f : now;
-            const uint64_t low = pair2(-base, -base), f2 = pair2(f, f);
+            const uint64_t low = pair2(-base, -base), f2 = pair2(f, f), keep = pair2(L::KEEP, L::KEEP);
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
               if (c) scores(c);  // the first half is still there
               uint32_t p[16];
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
-                // 0 at the largest, however large
-                const uint64_t d = mulf2(add2((uint64_t)x[i] | (uint64_t)x[i + 1] << 32, low), f2);
+                // KEEP at the largest, however large
+                const uint64_t d = fma2(add2((uint64_t)x[i] | (uint64_t)x[i + 1] << 32, low), f2, keep);
                 float y = exp2_fast(first2(d)), z = exp2_fast(second2(d));
                 if (!all) {
                   y = x[i] == 0xff800000u ? 0.0f : y;

@@ -13,8 +13,15 @@ rest of each beside it.)  Results then hold to test_gpu_pack's bounds, and
 more; h is 7 at least, where a row's first estimate of its largest is left
 standing while the largest grows by up to 2^8.
 
+Where a sequence has more than 16 query rows a key/value head, of 16 bits and at
+most 256 wide, keys are rounded to f16 too, and the score of a position that
+stands out is off by up to 2^-11 of it: the others' weights, and with them the
+result, by that factor.
+
 In the 2-norm f32 rows have the roundings of scores as large as `above`, each
 2^-24 of its partials, beside the 4e-6 of test_gpu_pack: 2^-22 `above`."""
+
+import math
 
 import pytest
 
@@ -42,7 +49,7 @@ def floor_of(s, window, sinks):
     return out
 
 
-def check(s, window=0, sinks=0, above=0.0):
+def check(s, window=0, sinks=0, above=0.0, rounded_keys=False):
     got = s.attend(window=window, sinks=sinks).double()
     want, tol = s.want(window, sinks)
     tol = tol + floor_of(s, window, sinks)
@@ -50,6 +57,8 @@ def check(s, window=0, sinks=0, above=0.0):
     over = ((got - want).abs() / tol).max().item()
     rel = ((got - want).norm() / want.norm()).item()
     norm = {torch.float32: 4e-6 + 2.0 ** -22 * above, torch.float16: 2.0 ** -11, torch.bfloat16: 2.3e-3}[s.kind]
+    if rounded_keys and s.kind != torch.float32:
+        norm += math.expm1(2.0 ** -11 * above)
     assert over <= 1.0 and rel <= norm, (over, rel)
     s.cache.status()
 
@@ -82,6 +91,18 @@ def test_first_positions_that_hold_the_weight(igc_lib, kind, above, window, rows
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,heads,size", [(40, 8, 256), (40, 8, 64), (24, 16, 128), (20, 7, 160)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("above", [10, 14])
+def test_first_positions_that_hold_the_weight_of_many_rows(igc_lib, kind, above, rows, heads, size):
+    """More units than blocks, so that most see the first positions and the
+    window behind them together."""
+    s = Setup(igc_lib, kind, [rows] * 60, [1400 + 7 * i for i in range(60)], heads, 1, size, seed=size + above)
+    stand_out(s, above)
+    check(s, window=900, sinks=4, above=above, rounded_keys=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,depth,heads,size", FEW + MANY)
 def test_first_positions_far_above_in_32_bits(igc_lib, rows, depth, heads, size):
     s = Setup(igc_lib, "f32", [rows], [depth], heads, 1, size, seed=size + rows)
@@ -93,10 +114,10 @@ def stand_out(s, above):
     """Columns 0 to 31 of every query are 1, and of the keys 7 scale in the
     first four positions and 0 in the others."""
     c = s.cache
-    slot = s.slot_list[0]
     s.q[:, :, :32] = 1.0
     s.q[:, :, 32:] *= 0.3
-    c.key_codes[slot, :, :, :16] = 0x88
-    c.key_codes[slot, :, :4, :16] = 0xFF
-    c.key_scales[slot, :, :4, 0] = above / (7 * 32 * s.size ** -0.5)
-    c.value_codes[slot, :, :4] = 0x88
+    for slot in s.slot_list:
+        c.key_codes[slot, :, :, :16] = 0x88
+        c.key_codes[slot, :, :4, :16] = 0xFF
+        c.key_scales[slot, :, :4, 0] = above / (7 * 32 * s.size ** -0.5)
+        c.value_codes[slot, :, :4] = 0x88
