@@ -128,6 +128,9 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
   uint16_t *scales = side ? a.c.vs : a.c.ks;
   const size_t col = (size_t)head * d.head_stride + PK_COLS * w;
   int row = blockIdx.x * (a.rows * PK_ITEMS * PK_TURNS) + r;
+  // every sequence that is not to be run is told, those that no row leads to among them
+  if (a.r.starts && blockIdx.y == 0)
+    for (int i = blockIdx.x * PK_THREADS + threadIdx.x; i < a.r.count; i += gridDim.x * PK_THREADS) seq_at(a.c, a.r, i);
   int s = a.r.starts ? seq_before(a.r, min(row - r, a.r.rows - 1)) : 0;
   if (r >= a.rows) return;  // threads past a whole number of rows
   SeqAt q = {0, 0, 0, -1};

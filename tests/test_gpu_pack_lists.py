@@ -1,0 +1,40 @@
+"""The packed cache's trouble word: what lists that do not fit set, in every
+call, and what a status leaves behind."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_pack import Setup  # noqa: E402
+
+# six rows; the list, the most rows of a sequence, and the rows that no sequence is run for
+BAD = [([0, 2, 4, 7], None, [4, 5]), ([0, 2, 4, 6, 9], None, []), ([0, 6, 2], None, []), ([0, 4, 2, 6], None, []),
+       ([0, 1, 5, 6], 3, [1, 2, 3, 4]), ([-1, 2, 4, 6], None, [0, 1]), ([0, 6, 6, 8], None, []),
+       ([0] + [6] * 400 + [7], None, [])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts,most,left", BAD)
+def test_lists_that_do_not_fit_are_told_by_every_call(igc_lib, starts, most, left):
+    n = len(starts) - 1
+    s = Setup(igc_lib, "bf16", [2, 2, 2], [10, 30, 20], 8, 1, 64, seed=1)
+    at = dict(starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), rows_most=most,
+              slots=s.slots[torch.arange(n, device="cuda") % 3].contiguous())
+    fill = (torch.arange(n, dtype=torch.int32, device="cuda") % 3) * 10 + 5
+    scales = s.cache.key_scales.clone()
+    s.cache.write(s.k, s.v, fill, **at)
+    with pytest.raises(igc_lib.IgcError) as e:
+        s.cache.status()
+    assert e.value.code == igc_lib.FAIL_STATE
+    s.cache.status()
+    out = torch.full_like(s.k, 5.0), torch.full_like(s.k, 5.0)
+    s.cache.read(fill, 6, torch.bfloat16, out=out, **at)
+    with pytest.raises(igc_lib.IgcError):
+        s.cache.status()
+    assert (out[0][left] == 5.0).all() and (out[1][left] == 5.0).all()
+    s.cache.attend(s.q, fill, scale=0.125, **at)
+    with pytest.raises(igc_lib.IgcError):
+        s.cache.status()
+    if len(left) == 4:  # of the sequence with too many rows nothing was written
+        slot = s.slot_list[1]
+        assert torch.equal(s.cache.key_scales[slot].view(torch.int16), scales[slot].view(torch.int16))
