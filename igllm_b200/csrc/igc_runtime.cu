@@ -3570,5 +3570,6 @@ extern "C" int igc_pack_status(const igc_pack *p, void *stream) {
   CK(cudaStreamSynchronize((cudaStream_t)stream));
   if (word == 0) return IGC_OKAY;
   CK(cudaMemsetAsync(p->trouble, 0, sizeof(word), (cudaStream_t)stream));
+  CK(cudaStreamSynchronize((cudaStream_t)stream));  // calls that come after this one, on any stream, set it for the next
   return IGC_FAIL_STATE;
 }

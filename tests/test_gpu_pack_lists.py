@@ -38,3 +38,17 @@ def test_lists_that_do_not_fit_are_told_by_every_call(igc_lib, starts, most, lef
     if len(left) == 4:  # of the sequence with too many rows nothing was written
         slot = s.slot_list[1]
         assert torch.equal(s.cache.key_scales[slot].view(torch.int16), scales[slot].view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_a_status_has_cleared_the_word_when_it_returns(igc_lib):
+    """Its clearing does not reach into calls that come after it on other
+    streams: nothing of it is left on its stream."""
+    s = Setup(igc_lib, "bf16", [1], [10], 8, 1, 64, seed=2)
+    lib, stream = igc_lib._lib(), torch.cuda.current_stream()
+    for _ in range(300):
+        s.cache._trouble.fill_(1)
+        code = lib.igc_pack_status(s.cache._p, stream.cuda_stream)
+        idle = stream.query()
+        assert code == igc_lib.FAIL_STATE and idle
+        assert lib.igc_pack_status(s.cache._p, stream.cuda_stream) == igc_lib.OKAY
