@@ -1285,7 +1285,9 @@ static int pack_room(igc_session *s, int lanes) {
   for (int l = 0; l < m->layers; ++l) {
     kv = std::max(kv, (size_t)m->layer[l].kv_rows);
     bool seen = false;  // layers of one shape plan alike
-    for (int o = 0; o < l; ++o) seen = seen || (m->layer[o].hd == m->layer[l].hd && m->layer[o].kind == m->layer[l].kind);
+    for (int o = 0; o < l; ++o)
+      seen = seen || (m->layer[o].hd == m->layer[l].hd && m->layer[o].kind == m->layer[l].kind &&
+                      m->layer[o].kv_heads == m->layer[l].kv_heads);
     for (int k = 1; k <= lanes && !seen; ++k) {
       PackPlan plan;
       CK(pack_layer_plan(s, l, k, &plan));
