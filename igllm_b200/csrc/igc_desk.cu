@@ -66,6 +66,14 @@ bool note(DeskState *s, int code) {
 
 bool ok(DeskState *s, cudaError_t e) { return note(s, e == cudaSuccess ? IGC_OKAY : IGC_FAIL_DEVICE); }
 
+// Host memory to the device on the desk's stream, there when this returns (a
+// plain cudaMemcpy's last bytes may still be on their way then, on a stream
+// that the desk's does not wait for).
+cudaError_t copy_in(DeskState *s, void *dst, const void *src, size_t bytes) {
+  const cudaError_t e = cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, s->st);
+  return e == cudaSuccess ? cudaStreamSynchronize(s->st) : e;
+}
+
 bool grow(DeskState *s, size_t floats) {
   if (floats <= s->buf_floats) return true;
   cudaFree(s->buf_a);
@@ -102,7 +110,7 @@ const DeskPlane *plain_plane_of(DeskState *s, const igc_plane *p, const void *ke
     if (!tb || !p->real_data) return void(note(s, IGC_FAIL_SUPPORT)), nullptr;
     const size_t bytes = (size_t)p->row_count * p->col_count * tb;
     if (!ok(s, cudaMalloc(&dp.plain_data, bytes)) ||
-        !ok(s, cudaMemcpy(dp.plain_data, p->real_data, bytes, cudaMemcpyHostToDevice)))
+        !ok(s, copy_in(s, dp.plain_data, p->real_data, bytes)))
       return nullptr;
     a.dense = dp.plain_data;
     a.dense_type = p->real_type;
@@ -133,8 +141,8 @@ const DeskPlane *plain_plane_of(DeskState *s, const igc_plane *p, const void *ke
     }
     const size_t cb = (size_t)p->row_count * p->row_stride;
     if (!ok(s, cudaMalloc(&dp.plain_data, cb)) || !ok(s, cudaMalloc(&dp.plain_scales, sizeof(float) * sc.size())) ||
-        !ok(s, cudaMemcpy(dp.plain_data, p->code_data, cb, cudaMemcpyHostToDevice)) ||
-        !ok(s, cudaMemcpy(dp.plain_scales, sc.data(), sizeof(float) * sc.size(), cudaMemcpyHostToDevice)))
+        !ok(s, copy_in(s, dp.plain_data, p->code_data, cb)) ||
+        !ok(s, copy_in(s, dp.plain_scales, sc.data(), sizeof(float) * sc.size())))
       return nullptr;
     a.codes = static_cast<const uint8_t *>(dp.plain_data);
     a.stride = p->row_stride;
@@ -177,8 +185,8 @@ const DeskPlane *plane_of(DeskState *s, const igc_plane *p) {
       !ok(s, cudaMalloc(&dp.scales, (size_t)dp.n_rb * dp.n_cc * 64)) || !ok(s, cudaMalloc(&dc, cb)) ||
       !ok(s, cudaMalloc(&ds, sb)))
     return nullptr;
-  bool good = ok(s, cudaMemcpy(dc, p->code_data, cb, cudaMemcpyHostToDevice)) &&
-              ok(s, cudaMemcpy(ds, sc.data(), sb, cudaMemcpyHostToDevice)) &&
+  bool good = ok(s, copy_in(s, dc, p->code_data, cb)) &&
+              ok(s, copy_in(s, ds, sc.data(), sb)) &&
               ok(s, igc_launch_repack(dc, p->row_stride, bits, ds, g32, p->row_count, p->col_count, dp.n_rb,
                                       dp.n_cc, 1, 0, dp.tiles, dp.scales, s->st)) &&
               ok(s, cudaStreamSynchronize(s->st));
@@ -288,7 +296,7 @@ void desk_mat_mat_lanes(DeskState *s, const DeskPlane *p, const float *act, int 
   int gave_up = 0;
   if (!ok(s, cudaMemcpy(&gave_up, s->err, sizeof(int), cudaMemcpyDeviceToHost))) return;
   if (gave_up) {
-    cudaMemset(s->err, 0, sizeof(int));
+    cudaMemsetAsync(s->err, 0, sizeof(int), s->st);
     note(s, IGC_FAIL_DEVICE);
   }
 }
@@ -343,7 +351,7 @@ void desk_mat_mat(igc_desk *d, const igc_plane *sheet, const float *act, int act
     int gave_up = 0;  // a projection that gave up waiting for its weight copies
     if (!ok(s, cudaMemcpy(&gave_up, s->err, sizeof(int), cudaMemcpyDeviceToHost))) return;
     if (gave_up) {
-      cudaMemset(s->err, 0, sizeof(int));
+      cudaMemsetAsync(s->err, 0, sizeof(int), s->st);
       return void(note(s, IGC_FAIL_DEVICE));
     }
     done += k;
@@ -409,7 +417,7 @@ extern "C" int igc_back_open(igc_desk *desk, int device) {
       igc_kernels_configure(227 * 1024) != cudaSuccess || igc_lanes_configure() != cudaSuccess ||
       cudaMalloc(&s->arg_val, (size_t)s->sm_count * 4 * 16 * 4) != cudaSuccess ||
       cudaMalloc(&s->arg_idx, (size_t)s->sm_count * 4 * 16 * 4) != cudaSuccess ||
-      cudaMalloc(&s->err, sizeof(int)) != cudaSuccess || cudaMemset(s->err, 0, sizeof(int)) != cudaSuccess) {
+      cudaMalloc(&s->err, sizeof(int)) != cudaSuccess || cudaMemsetAsync(s->err, 0, sizeof(int), s->st) != cudaSuccess) {
     delete s;
     return IGC_FAIL_DEVICE;
   }

@@ -62,6 +62,15 @@ static int fail_device(cudaError_t e, const char *where) {
     if (e_ != cudaSuccess) return fail_device(e_, #call); \
   } while (0)
 
+// Host memory to the device, there when this returns.  A plain cudaMemcpy from
+// pageable memory returns once the bytes are staged, with their copy still to
+// come on the default stream, which the library's own streams (non-blocking)
+// do not wait for: their kernels then read what lay there before.
+static cudaError_t copy_in(void *dst, const void *src, size_t bytes, cudaStream_t st) {
+  const cudaError_t e = cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, st);
+  return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
+}
+
 // An error a CUDA call left behind that its caller did not check would be
 // reported by the next launch check, against the wrong call.  Entry points
 // clear it first; IGC_DEBUG_ERRORS=1 names where a stale one was found.
@@ -452,7 +461,7 @@ struct Binder {
     for (size_t i = 0; i < n; ++i) host[i] = real_at(*t, i);
     int c = m->alloc(out, n);
     if (c != IGC_OKAY) return c;
-    CK(cudaMemcpy(*out, host.data(), n * sizeof(float), cudaMemcpyHostToDevice));
+    CK(copy_in(*out, host.data(), n * sizeof(float), st));
     m->decode_bytes += n * sizeof(float);
     m->weight_bytes += t->bytes;
     src.release(name);
@@ -569,8 +578,8 @@ struct Binder {
     c = m->alloc(&codes, v.code->bytes);
     if (c == IGC_OKAY) c = m->alloc(&scales, sc.size());
     if (c != IGC_OKAY) return c;
-    CK(cudaMemcpy(codes, v.code->data, v.code->bytes, cudaMemcpyHostToDevice));
-    CK(cudaMemcpy(scales, sc.data(), sizeof(uint16_t) * sc.size(), cudaMemcpyHostToDevice));
+    CK(copy_in(codes, v.code->data, v.code->bytes, st));
+    CK(copy_in(scales, sc.data(), sizeof(uint16_t) * sc.size(), st));
     out.codes = codes;
     out.stride = (size_t)v.code->shape[1];
     out.bits = v.bits;
@@ -606,7 +615,7 @@ struct Binder {
         void *d = nullptr;
         int c = m->alloc(reinterpret_cast<uint8_t **>(&d), p.dense->bytes);
         if (c != IGC_OKAY) return c;
-        CK(cudaMemcpy(d, p.dense->data, p.dense->bytes, cudaMemcpyHostToDevice));
+        CK(copy_in(d, p.dense->data, p.dense->bytes, st));
         a.dense = d;
         a.dense_type = p.dense->dtype;  // the reference's store types: 1 F32, 2 F16, 3 BF16
         counted = p.dense->bytes;
@@ -619,8 +628,8 @@ struct Binder {
         int c = m->alloc(&codes, p.code->bytes);
         if (c == IGC_OKAY) c = m->alloc(&scales, sc.size());
         if (c != IGC_OKAY) return c;
-        CK(cudaMemcpy(codes, p.code->data, p.code->bytes, cudaMemcpyHostToDevice));
-        CK(cudaMemcpy(scales, sc.data(), sizeof(float) * sc.size(), cudaMemcpyHostToDevice));
+        CK(copy_in(codes, p.code->data, p.code->bytes, st));
+        CK(copy_in(scales, sc.data(), sizeof(float) * sc.size(), st));
         a.codes = codes;
         a.stride = (size_t)p.code->shape[1];
         a.bits = p.bits;
@@ -675,8 +684,8 @@ struct Binder {
       if (c != IGC_OKAY) return c;
       CK(cudaMalloc(&dc, cb));
       CK(cudaMalloc(&ds, sizeof(uint16_t) * sc.size()));
-      CK(cudaMemcpy(dc, p.code->data, cb, cudaMemcpyHostToDevice));
-      CK(cudaMemcpy(ds, sc.data(), sizeof(uint16_t) * sc.size(), cudaMemcpyHostToDevice));
+      CK(copy_in(dc, p.code->data, cb, st));
+      CK(copy_in(ds, sc.data(), sizeof(uint16_t) * sc.size(), st));
       int prb = (p.rows + 15) / 16;
       int mul = pair ? 2 : 1, add = pair ? (int)k : rb_at;
       cudaError_t e = igc_launch_repack(dc, (size_t)p.code->shape[1], p.bits, ds, (p.cols + 31) / 32, p.rows, p.cols,
@@ -739,7 +748,7 @@ struct Binder {
     if (cols > 0 && t->shape[1] != cols) return IGC_FAIL_FORMAT;
     int c = m->alloc(out, t->bytes / 2);
     if (c != IGC_OKAY) return c;
-    CK(cudaMemcpy(*out, t->data, t->bytes, cudaMemcpyHostToDevice));
+    CK(copy_in(*out, t->data, t->bytes, st));
     *rows_out = (int)t->shape[0];
     m->decode_bytes += (size_t)t->shape[1] * 2; /* app_core.c:1880 plane_row_bytes */
     m->weight_bytes += t->bytes;
@@ -761,7 +770,7 @@ static int build_rope(igc_model *m, int kind, int hd, cudaStream_t st) {
     if (!r.proportional || i < turn) steps[i] = (float)(1.0 / pow(r.theta, (double)(2 * i) / (double)hd));
   float *d_steps = nullptr;
   CK(cudaMalloc(&d_steps, sizeof(float) * (size_t)half));
-  CK(cudaMemcpy(d_steps, steps.data(), sizeof(float) * (size_t)half, cudaMemcpyHostToDevice));
+  CK(copy_in(d_steps, steps.data(), sizeof(float) * (size_t)half, st));
   int c = m->alloc(&m->rope_cs[kind], (size_t)m->window_limit * half);
   if (c == IGC_OKAY) c = m->alloc(&m->rope_sn[kind], (size_t)m->window_limit * half);
   if (c != IGC_OKAY) { cudaFree(d_steps); return c; }
@@ -2202,8 +2211,8 @@ static int chunks_ready(igc_session *s) {
       hv[(size_t)l * C.groups_cap + z] = attn_rows(s, owner, 1);
     }
   }
-  CK(cudaMemcpy(C.kc_tab, hk.data(), sizeof(float *) * hk.size(), cudaMemcpyHostToDevice));
-  CK(cudaMemcpy(C.vc_tab, hv.data(), sizeof(float *) * hv.size(), cudaMemcpyHostToDevice));
+  CK(copy_in(C.kc_tab, hk.data(), sizeof(float *) * hk.size(), s->st));
+  CK(copy_in(C.vc_tab, hv.data(), sizeof(float *) * hv.size(), s->st));
   CK(cudaMallocHost(&C.h_ids, sizeof(int32_t) * (1 + M)));
   return IGC_OKAY;
 }
@@ -2801,7 +2810,7 @@ extern "C" int igc_crowd_open(igc_model *m, int session_limit, int lanes_per_ses
   CK(cudaMalloc(&v, sizeof(int32_t) * (cr->lanes + 1)));
   cr->owned.push_back(v);
   cr->d_top = (int32_t *)v;
-  CK(cudaMemset(cr->d_top, 0, sizeof(int32_t) * (cr->lanes + 1)));
+  CK(cudaMemsetAsync(cr->d_top, 0, sizeof(int32_t) * (cr->lanes + 1), cr->st));
   CK(cudaMallocHost(&v, cr->tab_bytes));
   cr->h_tab = (uint8_t *)v;
   CK(cudaMallocHost(&v, sizeof(int32_t) * (cr->lanes + 1)));
@@ -3236,7 +3245,7 @@ extern "C" int igc_session_bench(igc_session *s, const int32_t *blocks, int roun
     host[r * rec] = s->fill + r * k;
     memcpy(&host[r * rec + 1], blocks + (size_t)r * k, sizeof(int32_t) * k);
   }
-  CK(cudaMemcpy(s->d_rounds, host.data(), sizeof(int32_t) * host.size(), cudaMemcpyHostToDevice));
+  CK(copy_in(s->d_rounds, host.data(), sizeof(int32_t) * host.size(), s->st));
   // the pass of this shape, captured once
   if (s->use_graphs && !s->graph[k][1]) {
     CK(cudaMemcpyAsync(s->d_io, s->d_rounds, sizeof(int32_t) * rec, cudaMemcpyDeviceToDevice, s->st));
