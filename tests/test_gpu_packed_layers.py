@@ -1,4 +1,4 @@
-"""Packed sessions of models whose layers are not alike."""
+"""Packed sessions of models whose layers are not alike, and of wide heads."""
 
 import json
 import os
@@ -7,7 +7,8 @@ import struct
 import numpy as np
 import pytest
 
-from conftest import SMALL
+from conftest import SMALL, make_checkpoint
+from test_gpu_packed_session import ATOL, Drawn
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +59,25 @@ def test_layers_of_several_key_head_counts(igc_lib, tmp_path):
         rows[-1].append(s.step(ids[21])[1].copy()[None])
     for a, b in zip(*rows):
         assert np.isfinite(a).all() and np.abs(a - b).max() <= 2e-2
+
+
+def test_wide_heads_against_the_restatement(igc_lib, igo_mod, tmp_path):
+    """512-wide heads on every layer, sliding and global: a prompt, blocks and
+    steps, every row of them to the parity bar."""
+    cfg = dict(SMALL, heads=4, head_dim=512, slide_span=40, window_limit=1024)
+    folder = str(tmp_path / "wide")
+    make_checkpoint(igc_lib, folder, cfg)
+    d = Drawn(igo_mod, folder, cfg, 2, 8)
+    m = igc_lib.Model(folder=folder, window_limit=cfg["window_limit"])
+    s = igc_lib.Session(m, packed=True, sinks=2)
+    ids = d.tokens(140)
+    s.prime(ids)
+    d.o.prime(ids)
+    for k in (1, 5, 16):
+        blk = d.tokens(k)
+        got, want = s.guess(blk), d.o.guess(blk)
+        assert np.abs(got - want).max() <= ATOL
+        s.guess_keep(k)
+        d.o.guess_keep(k)
+        t = d.tokens(1)[0]
+        assert np.abs(s.step(t)[1] - d.o.step(t)).max() <= ATOL
