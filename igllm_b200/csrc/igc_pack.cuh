@@ -272,20 +272,28 @@ __device__ __forceinline__ int seq_weight(const PackAttend &a, int s, int rb, in
 }
 
 // Every warp finds its place by itself: 32 sequences at a time, or (tall)
-// sequence by sequence 32 of its blocks at a time.
+// sequence by sequence 32 of its blocks at a time.  -1 where the list weighs
+// more than list_most, as a list of starts that goes back and forth gives rows
+// to many sequences: none of it is run, which bounds what a call does and keeps
+// every sum in 31 bits (a sequence's weight is below list_most, a lane's sum
+// below twice that, and the warp's is first taken in 64ths).
 __device__ __forceinline__ int list_total(const PackAttend &a, int rb, int tp, int over, int tall) {
   const int lane = threadIdx.x & 31;
-  int w = 0;
+  uint32_t w = 0;
+  const uint32_t most = (uint32_t)a.list_most;
   if (!tall) {
-    for (int i = lane; i < a.r.count; i += 32) w += seq_weight(a, i, rb, tp, over);
+    for (int i = lane; i < a.r.count; i += 32) w = min(w, most) + (uint32_t)seq_weight(a, i, rb, tp, over);
   } else {
     for (int s = 0; s < a.r.count; ++s) {
       const SeqAt q = seq_at(a.c, a.r, s);
       const int nb = blocks_of(a, q, rb);
-      for (int b = lane; b < nb; b += 32) w += unit_weight(a, q, b, rb, tp, over) * a.c.heads;
+      for (int b = lane; b < nb; b += 32) w = min(w, most) + (uint32_t)(unit_weight(a, q, b, rb, tp, over) * a.c.heads);
+      if (__any_sync(0xffffffffu, w > most)) break;
     }
   }
-  return __reduce_add_sync(0xffffffffu, w);
+  if (__reduce_add_sync(0xffffffffu, w >> 6) > (most >> 6)) return -1;
+  w = __reduce_add_sync(0xffffffffu, w);
+  return w > most ? -1 : (int)w;
 }
 
 // Among 32 weights, a lane each, after `before` in all: the lane that holds
@@ -355,6 +363,7 @@ __device__ __forceinline__ bool walk_start(const PackAttend &a, int tall, PackWa
   *share_out = share;
   w.at = blockIdx.x * share;
   w.end = min(total, w.at + share);
+  if (total < 0) pack_trouble(a.c);
   if (w.at >= w.end) return false;
   int before = 0, l = -1;
   if (!tall) {

@@ -59,6 +59,7 @@ struct PackAttend {
   int window, sinks;  // window 0: every position up to the row's own
   float scale;
   float *work;        // split units' partial sums (PackPlan::work_floats)
+  int list_most;      // PackPlan::list_most
 };
 
 // How a call's attention runs, from its host-known sizes alone.
@@ -74,6 +75,7 @@ struct PackPlan {
   int tall;      // some sequence has many blocks of rows; with clusters, the most of any
   int cluster;   // blocks of a cluster that share a unit, 0: the list of tiles instead
   int grid;
+  int list_most;  // the most the list of tiles weighs where no two sequences hold one row
   size_t work_floats;
 };
 

@@ -1342,7 +1342,8 @@ static int pack_attend(igc_session *s, int l, const float *qkv, const int *p0, i
                         sliding ? m->slide_span : 0,
                         sliding ? s->sinks : 0,
                         1.0f,  // app_core.c:11314: the norms carry the scale
-                        s->pack_work};
+                        s->pack_work,
+                        plan.list_most};
   int launches = 0;
   const cudaError_t e = igc_launch_pack_attend(&a, &plan, s->st, &launches);
   g_launches += launches;
@@ -3562,7 +3563,8 @@ extern "C" int igc_pack_attend(const igc_pack *p, const igc_pack_rows *rows, int
   if (int c = pack_plan_of(p, r, heads, q->real_type, window, sinks, &plan)) return c;
   if (plan.work_floats * sizeof(float) > work_bytes || (plan.work_floats && !work)) return IGC_FAIL_MEMORY;
   const PackAttend a = {pack_view(p), r,     pack_data_of(q), pack_data_of(out), heads / p->head_count,
-                        Quotient::by(heads / p->head_count), window,       sinks, scale,           (float *)work};
+                        Quotient::by(heads / p->head_count), window,       sinks, scale,           (float *)work,
+                        plan.list_most};
   int launches = 0;
   const cudaError_t e = igc_launch_pack_attend(&a, &plan, (cudaStream_t)stream, &launches);
   g_launches += launches;

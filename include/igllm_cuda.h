@@ -375,8 +375,10 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * A row at a negative position is padding: not written, and zeros out.  A row
  * at position_count or beyond, or of a slot the cache lacks, is not written,
  * comes out as zeros and sets the trouble word; a sequence whose rows fall
- * outside [0, row_count) or pass rows_most is not run and sets it too.  The
- * places written by one call are the caller's to keep distinct.
+ * outside [0, row_count) or pass rows_most is not run and sets it too, and
+ * where starts go back and forth, so that the sequences hold more rows together
+ * than there are, an attention may run none.  The places written by one call
+ * are the caller's to keep distinct.
  *
  * igc_pack_data is an array of rows: `real_type` 1 F32, 2 F16, 3 BF16 (the
  * reference's store_type values), strides in values, a head's values adjacent;

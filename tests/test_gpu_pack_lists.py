@@ -52,3 +52,26 @@ def test_a_status_has_cleared_the_word_when_it_returns(igc_lib):
         idle = stream.query()
         assert code == igc_lib.FAIL_STATE and idle
         assert lib.igc_pack_status(s.cache._p, stream.cuda_stream) == igc_lib.OKAY
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [4, 600])
+def test_starts_back_and_forth_do_not_multiply_the_work(igc_lib, kind, rows):
+    """Every second sequence holds all rows: a list of 2^31 tiles and more from
+    a call whose sizes allow a few thousand.  None of it is run, and it is told."""
+    heads, n = 8, 40000
+    cache = igc_lib.PackCache.open(1, heads, 1 << 20, 32)
+    dtype = {"f32": torch.float32, "bf16": torch.bfloat16}[kind]
+    q = torch.randn(rows, 5 * heads, 32, device="cuda").to(dtype)
+    starts = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    starts[1::2] = rows
+    at = dict(starts=starts, slots=torch.zeros(n, dtype=torch.int32, device="cuda"))
+    fill = torch.full((n,), (1 << 20) - rows, dtype=torch.int32, device="cuda")
+    out = cache.attend(q, fill, out=torch.full_like(q, 5.0), **at)
+    with pytest.raises(igc_lib.IgcError) as e:
+        cache.status()
+    assert e.value.code == igc_lib.FAIL_STATE and (out == 5.0).all()
+    out = cache.attend(q, fill[:1], starts=starts[:2].contiguous(), slots=at["slots"][:1], out=out)
+    cache.status()
+    assert out.abs().max() == 0  # a cleared cache
