@@ -1122,7 +1122,7 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   const long blocks = (need + rb - 1) / rb, tiles = most_tiles(p, rb, positions, group, window, sinks);
   // no more units than whole blocks and a part of one for each sequence that has rows
   const double list = ((double)rows * group / rb + (count < rows ? count : rows)) * kv_heads * (tiles + p->over);
-  if (list >= 2147418112.0) return cudaErrorInvalidValue;  // 31 bits, with room for a share's rounding
+  if (list >= 2147418112.0) return cudaErrorNotSupported;  // 31 bits, with room for a share's rounding
   p->list_most = (int)list + 1;
   // blocks of at least 7 steps, were all units as long as they can be: shorter runs
   // leave more pieces to join than they save (one token at 32000: 49 us by single

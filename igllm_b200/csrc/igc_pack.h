@@ -86,7 +86,8 @@ cudaError_t igc_launch_pack_write(const igc::PackView *c, const igc::PackRows *r
                                   const igc::PackData *v, cudaStream_t st);
 cudaError_t igc_launch_pack_read(const igc::PackView *c, const igc::PackRows *r, const igc::PackData *k,
                                  const igc::PackData *v, cudaStream_t st);
-// `type` the query rows' type, `rows_most` the most rows of any sequence.
+// `type` the query rows' type, `rows_most` the most rows of any sequence;
+// cudaErrorNotSupported where the call's tiles are too many to count.
 cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int kv_heads, int group, int size,
                           int type, int window, int sinks, igc::PackPlan *plan);
 // igc_pack_tc.cu's part of the two calls around it.

@@ -3516,8 +3516,10 @@ bool pack_attend_sane(const igc_pack *p, const igc_pack_rows *rows, int heads, i
 }
 
 int pack_plan_of(const igc_pack *p, const PackRows &r, int heads, int type, int window, int sinks, PackPlan *plan) {
-  CK(igc_pack_plan(r.count, r.rows, r.most, p->position_count, p->head_count, heads / p->head_count, p->head_size, type,
-                   window, sinks, plan));
+  const cudaError_t e = igc_pack_plan(r.count, r.rows, r.most, p->position_count, p->head_count, heads / p->head_count,
+                                      p->head_size, type, window, sinks, plan);
+  if (e == cudaErrorNotSupported) return IGC_FAIL_SUPPORT;
+  CK(e);
   return IGC_OKAY;
 }
 

@@ -396,7 +396,9 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * a row, and for F32 rows every product keeps both halves of a hi/lo split, so
  * that results hold to f32.  `work` is device scratch of at least the bytes
  * igc_pack_attend_room gives for the same arguments (often none; a multiple of 16 bytes
- * aligned); calls that may run at once need scratch of their own.
+ * aligned); calls that may run at once need scratch of their own.  A call whose
+ * rows and positions come to 2^31 tiles or more, were all rows at the cache's
+ * end, is refused with IGC_FAIL_SUPPORT.
  *
  * Each call makes pack->device current and restores the caller's device; work
  * is queued on `stream` (a cudaStream_t, NULL the default stream) and not

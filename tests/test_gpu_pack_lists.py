@@ -1,6 +1,8 @@
 """The packed cache's trouble word: what lists that do not fit set, in every
 call, and what a status leaves behind."""
 
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -75,3 +77,14 @@ def test_starts_back_and_forth_do_not_multiply_the_work(igc_lib, kind, rows):
     out = cache.attend(q, fill[:1], starts=starts[:2].contiguous(), slots=at["slots"][:1], out=out)
     cache.status()
     assert out.abs().max() == 0  # a cleared cache
+
+
+@pytest.mark.gpu
+def test_a_call_of_too_many_tiles_is_refused_as_such(igc_lib):
+    """2^24 rows over 2^20 positions of 8 heads: no pointer is followed."""
+    pack = igc_lib.IgcPack(4096, 4096, 4096, 4096, 1, 8, 1 << 20, 64, 0, None)
+    room = ctypes.c_size_t(5)
+    for rows, want in ((1 << 24, igc_lib.FAIL_SUPPORT), (1 << 12, igc_lib.OKAY)):
+        r = igc_lib.IgcPackRows(1, rows, 0, None, 4096, None)
+        for kind in (1, 2, 3):
+            assert igc_lib._lib().igc_pack_attend_room(pack, r, 8, kind, 0, 0, room) == want
