@@ -666,7 +666,7 @@ class PackCache:
         self.slots, self.heads, self.positions, self.size = slots, heads, positions, 2 * half
         self.key_codes, self.key_scales = key_codes, key_scales
         self.value_codes, self.value_scales = value_codes, value_scales
-        self._trouble = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._trouble = self._clear_word(torch, self.device)
         self._p = IgcPack(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
                           value_scales.data_ptr(), slots, heads, positions, 2 * half, self.device.index,
                           self._trouble.data_ptr())
@@ -680,6 +680,23 @@ class PackCache:
         if positions % PACK_TILE or self.size % PACK_GROUP or not PACK_GROUP <= self.size <= 512:
             raise ValueError(f"PackCache: {positions} positions (a multiple of {PACK_TILE}) of {self.size} values "
                              f"(a multiple of {PACK_GROUP} up to 512)")
+
+    _own_streams = {}  # by device
+
+    @classmethod
+    def _clear_word(cls, torch, device):
+        """A zero that is there when this returns, whichever stream the first
+        call is on, and with no wait for what the current stream has queued."""
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return torch.zeros(1, dtype=torch.int32, device=device)
+            stream = cls._own_streams.get(device)
+            if stream is None:
+                stream = cls._own_streams[device] = torch.cuda.Stream(device)
+            with torch.cuda.stream(stream):
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+            stream.synchronize()
+        return word
 
     @classmethod
     def open(cls, slots, heads, positions, size, device=0):
