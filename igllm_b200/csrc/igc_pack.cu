@@ -240,9 +240,9 @@ __global__ void __launch_bounds__(PK_THREADS) pack_rows_kernel(const __grid_cons
 // the tensor core's sums round towards zero.
 //
 // Bound by instruction issue: four query heads over 131071 positions of 8 x 128
-// take 56 us (151 MB: 2.7 TB/s, issue 65% busy), 512 rows of 8 heads of 512
-// over 8704 positions 353 us (200 TFLOP/s, 37% of the tensor pipe), 511 f32 rows
-// behind a window of 512 44 us, one token at 1024 9 us.  Steps are 128 positions
+// take 57 us (151 MB: 2.7 TB/s, issue 64% busy), 512 rows of 8 heads of 512
+// over 8704 positions 347 us (204 TFLOP/s, 38% of the tensor pipe), 511 f32 rows
+// behind a window of 512 46 us, one token at 1024 9 us.  Steps are 128 positions
 // for 8 and 16 rows to 256 wide; wider tiles' registers leave room for 64.
 
 template <int HDP, int NT, bool SP>
@@ -1124,9 +1124,10 @@ cudaError_t igc_pack_plan(int count, int rows, int rows_most, int positions, int
   const double list = ((double)rows * group / rb + (count < rows ? count : rows)) * kv_heads * (tiles + p->over);
   if (list >= 2147418112.0) return cudaErrorNotSupported;  // 31 bits, with room for a share's rounding
   p->list_most = (int)list + 1;
-  // blocks of at least 7 steps, were all units as long as they can be: shorter runs
-  // leave more pieces to join than they save (one token at 32000: 49 us by single
-  // steps, 29 by 4, 28 by 7; 100000: 60, 60, 53)
+  // blocks of at least 7 steps, were all units as long as the cache's room lets them
+  // be (their depths are on the device; in a roomier cache the runs are shorter):
+  // shorter runs leave more pieces to join than they save (one token at 32000 in a
+  // cache of that room: 49 us by single steps, 29 by 4, 28 by 7; 100000: 60, 60, 53)
   p->grid = sms * per_sm;
   if (list / 7 < p->grid) p->grid = list < 7 ? 1 : (int)(list / 7);
   p->tall = blocks > 8;

@@ -35,8 +35,8 @@
 // cycles (64 positions wide: 61% of the pipe's rate) and 4 value products of 129
 // (all of it), 1360 cycles; warp 16 is busy 1400 to 1540 a step.  Wider score
 // products would need 128 rows of key operands twice, which the queries leave no
-// room for.  3 prompts to 4096 of 8 x 256: 122 us, 640 TFLOP/s; 8192 rows behind
-// a window of 512: 100 us; 64 x 4 rows at 8192: 66 us.  The mma.sync form took
+// room for.  3 prompts to 4096 of 8 x 256: 124 us, 630 TFLOP/s; 8192 rows behind
+// a window of 512: 101 us; 64 x 4 rows at 8192: 66 us.  The mma.sync form took
 // 506, 355 and 104.  A unit's ends (queries in, results out) cost about 8 steps,
 // which OVER tells the sharing (4, 7 and 10 measured: 64 x 4 in 86, 81 and 83 us,
 // prompts in 164, 127 and 131, before the joining was sped up).

@@ -394,7 +394,11 @@ int igc_norm_rms_fixed(int device, const float *value_list, const float *gain_li
  * is read from the cache: write it first.  `out` has the queries' type.  Sums
  * and the softmax are f32; queries are read as f16 after an exact power of two
  * a row, and for F32 rows every product keeps both halves of a hi/lo split, so
- * that results hold to f32.  `work` is device scratch of at least the bytes
+ * that results hold to f32.  For F16 and BF16 rows weights and values enter the
+ * products as f16, each off by 2^-11 of itself at most (a weight below 2^-21 of
+ * its row's largest by 2^-32 of the largest), and where a sequence has more
+ * than 16 rows a key/value head, of heads up to 256 wide, keys may too: a score
+ * is then off by up to 2^-11 scale sum |q||k|.  `work` is device scratch of at least the bytes
  * igc_pack_attend_room gives for the same arguments (often none; a multiple of 16 bytes
  * aligned); calls that may run at once need scratch of their own.  A call whose
  * rows and positions come to 2^31 tiles or more, were all rows at the cache's
